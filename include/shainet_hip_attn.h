@@ -206,6 +206,94 @@ int shainet_kv_cache_lengths_from_device(shainet_kv_cache *cache);
 int shainet_attn_decode_step(shainet_attn_ctx *ctx, shainet_kv_cache *cache, int n_seqs, const float *q,
                              const float *k, const float *v, float *out);
 
+/* ---- a cache in pages ------------------------------------------------------
+ *
+ * shainet_kv_cache reserves its capacity for every sequence ahead.  Here sequences take pages of page_rows rows
+ * as they grow and give them back as they shrink, so that a server's memory holds as many rows as its requests
+ * have.  For each of `layers` layers K and V are [n_pages][num_kv_heads][page_rows][head_dim] of float32, bfloat16
+ * or float16 numbers (rows are rounded once, when they are placed; queries, sums and outputs are float32), and
+ * all layers share, on the device,
+ *   table [n_seqs][seq_pages]   the page of each page_rows rows of a sequence; entries behind its last page: anything
+ *   lens [n_seqs]               rows of each sequence
+ *   free_pages [n_pages]        a stack: its first *n_free entries are the pages that nobody holds
+ * so that the host need not know where a row lies, nor how many there are.  No counterpart in the reference.
+ *
+ * head_dim a multiple of 8 up to 256, page_rows a power of two in 8..1024, n_seqs up to SHAINET_HIP_MAX_PAGED_SEQS;
+ * n_pages * page_rows, n_seqs * seq_pages below 2^31, seq_pages * page_rows below 2^30.  The context gives the head
+ * geometry and the stream and must outlive the cache; contexts of other layers may use the cache too, with
+ * the same kv heads and head_dim, at most as many query heads, and the same stream (shainet_attn_set_stream).
+ * Calls that rotate rows extend their context's cos/sin table to seq_pages * page_rows positions the first time, which waits
+ * and cannot be recorded (SHAINET_HIP_ERR_ARGUMENT then); otherwise calls allocate nothing unless they say so.  Calls are made
+ * with the device current that was current at creation.  One caller at a time per cache. */
+#define SHAINET_HIP_PAGE_F32 0
+#define SHAINET_HIP_PAGE_BF16 1
+#define SHAINET_HIP_PAGE_F16 2
+#define SHAINET_HIP_MAX_PAGED_SEQS 4096
+typedef struct shainet_paged_cache shainet_paged_cache;
+int shainet_paged_cache_create(shainet_paged_cache **out, shainet_attn_ctx *ctx, int layers, int n_pages, int page_rows,
+                               int n_seqs, int seq_pages, int dtype);
+int shainet_paged_cache_destroy(shainet_paged_cache *cache);
+/* Device addresses of the arrays above (K and V of one layer); any of the outputs may be null.  A caller that writes to
+ * them itself (pages that sequences share, a table of its own scheduler) keeps that ordered with the context's stream and
+ * calls shainet_paged_cache_lengths_from_device afterwards.  Kernels look at no page outside the pool, whatever the table says:
+ * keys whose page is none of the n_pages take no part. */
+int shainet_paged_cache_arrays(shainet_paged_cache *cache, int layer, void **k, void **v, int **table, int **lens,
+                               int **free_pages, int **n_free);
+
+/* The lengths of n sequences change by delta[i] rows (device arrays; seq_ids null: sequences 0..n-1): pages are taken
+ * and given back, and for each row gained, in the entries' order, slots[r] = page * page_rows + row in the page,
+ * positions[r] and row_seqs[r] are written (device arrays of max_rows entries; those behind the last row become -1).
+ * Pages given back in a call can be taken in it; a call followed by its inverse leaves the stack as it was.
+ * Asynchronous on the context's stream, depends on nothing but its arguments: can be recorded and replayed.  All or nothing: a sequence out of range or named twice, a length below 0, or too few pages, too
+ * narrow a table or too many rows for the lists leave lengths, table and stack as they were and all three lists at -1;
+ * the next shainet_attn_sync or shainet_paged_cache_lengths_from_device then returns SHAINET_HIP_ERR_ARGUMENT or
+ * SHAINET_HIP_ERR_CAPACITY. */
+int shainet_paged_cache_map_rows(shainet_paged_cache *cache, const int *seq_ids, const int *delta, int n, int *slots,
+                                 int *positions, int *row_seqs, int max_rows);
+/* After calls that change lengths on the device (map_rows, step_paged, or replays of them) the host's copy is stale and
+ * shainet_attn_forward_paged, truncate, read and the two calls for numbers are refused (-1) until this one, which waits. */
+int shainet_paged_cache_lengths_from_device(shainet_paged_cache *cache);
+int shainet_paged_cache_len(const shainet_paged_cache *cache, int seq);
+int shainet_paged_cache_free_pages(const shainet_paged_cache *cache);
+/* Drop the rows at positions >= len and give their pages back; clear: all rows, of every sequence when seq < 0 (then whether
+ * or not the host knows the lengths, and with page 0 the next to be taken). */
+int shainet_paged_cache_truncate(shainet_paged_cache *cache, int seq, int len);
+int shainet_paged_cache_clear(shainet_paged_cache *cache, int seq);
+/* Rows pos0 .. pos0+n-1 of one kv head of one sequence, as floats, to host buffers ([n][head_dim] each; either may be null). */
+int shainet_paged_cache_read(shainet_paged_cache *cache, int layer, int seq, int kv_head, int pos0, int n, float *k_out,
+                             float *v_out);
+
+/* Bias, QK-norm and RoPE of `rows` rows of q, k and v (device pointers, rows at the given strides), as shainet_attn_forward
+ * does them: rotated queries to q_rot [rows, num_heads*head_dim], K and V rows to slots[row], rotated by positions[row].
+ * Rows whose slot is no slot of the cache or whose position is outside the cos/sin table (those of a map at -1) are left
+ * alone, in q_rot too.  Slots are distinct.  Asynchronous on the context's stream. */
+int shainet_attn_append_paged(shainet_attn_ctx *ctx, shainet_paged_cache *cache, int layer, const int *slots,
+                              const int *positions, int rows, const float *q, long long q_stride, const float *k,
+                              long long k_stride, const float *v, long long v_stride, float *q_rot);
+/* Grouped-query attention of row r (rotated queries, 1/sqrt(head_dim) applied here) over the first positions[r] + 1 rows of
+ * sequence row_seqs[r], by the table (the lengths are not looked at; several rows may name one sequence).  A row with
+ * row_seqs outside 0..n_seqs-1 leaves its output alone; one with positions < 0, or whose keys' pages are all outside the
+ * pool, gets zeros.  At most SHAINET_HIP_MAX_PAGED_SEQS rows.  Rows of q_rot and out at the given strides.  Asynchronous on the
+ * context's stream.  Scores, softmax and sums are float32; the keys and values of the pages' numbers as
+ * they are.  Replays of recordings that use one cache must not overlap. */
+int shainet_attn_attend_paged(shainet_attn_ctx *ctx, shainet_paged_cache *cache, int layer, const int *row_seqs,
+                              const int *positions, int rows, const float *q_rot, long long q_stride, float *out,
+                              long long out_stride);
+/* A decode step: one new row for each of n sequences (seq_ids: device array, null: sequences 0..n-1); map, append and attend
+ * with lists of the cache's own.  q [n, num_heads*head_dim], k, v [n, num_kv_heads*head_dim], out like q, device pointers.
+ * Layer 0 maps the rows; calls for the layers behind it use that map.  Can be recorded and replayed.  A step that found no
+ * room leaves `out` alone (see map_rows). */
+int shainet_attn_step_paged(shainet_attn_ctx *ctx, shainet_paged_cache *cache, int layer, const int *seq_ids, int n,
+                            const float *q, const float *k, const float *v, float *out);
+/* shainet_attn_forward over a cache in pages: any number of new rows for each of up to SHAINET_HIP_MAX_BATCH sequences (host
+ * arrays seq_ids and new_tokens), planned on the host, which must know the lengths.  Sequences with more than a few new rows
+ * have their pages gathered into one piece of float32 scratch (which grows on demand) first and run as any prompt does.  Layer 0 maps and counts
+ * the rows; calls for the layers behind it give the same seq_ids and new_tokens.  SHAINET_HIP_ERR_CAPACITY, and
+ * nothing appended, when a sequence would outgrow its table or the pages do not suffice. */
+int shainet_attn_forward_paged(shainet_attn_ctx *ctx, shainet_paged_cache *cache, int layer, const int *seq_ids,
+                               const int *new_tokens, int n_seqs, const float *q, const float *k, const float *v,
+                               float *out, int mem);
+
 /* Copy of the rotated query rows of the last shainet_attn_forward call
  * ([sum new_tokens, num_heads*head_dim], host): lets a test check RoPE positions
  * and QK-norm of Q exactly (llama_block.cr:332-344). */

@@ -110,6 +110,11 @@ int shainet_attn_create_unrotated(shainet_attn_ctx **out, int num_heads, int num
 int shainet_attn_run_biased(shainet_attn_ctx *c, shainet_kv_cache *kc, const float *q, const shainet::DistanceBias &bias,
                             int start_pos, int new_tokens, float *out);
 
+// Attention of new_tokens rotated queries at positions start_pos .. over one sequence's rows, which lie in [KV][cap][hd] arrays
+// of the caller's, the new ones among them.  Asynchronous on c's stream.
+int shainet_attn_run_rows(shainet_attn_ctx *c, const float *q_rot, float *k, float *v, int cap, int start_pos, int new_tokens,
+                          float *out);
+
 // Room for new_rows more rows of one sequence: drops rows that no later position can see (windowed
 // contexts), else grows the buffers.  keep_back: rows that a later truncate may take back, at most;
 // the rows those positions see stay too.

@@ -14,6 +14,7 @@
 #include "attn_context.hpp"
 #include "attn_kernels.hpp"
 #include "block_kernels.hpp"
+#include "paged.hpp"
 
 using namespace shainet;
 
@@ -54,6 +55,14 @@ int check_error_word(int *w) {
   if (!w || *(volatile int *)w == 0) return SHAINET_HIP_OK;
   const int what = *(volatile int *)w;
   *(volatile int *)w = 0;
+  if (what == kMapNoRoom)
+    return fail(SHAINET_HIP_ERR_CAPACITY,
+                "a map of new rows found too few free pages, a sequence at the end of its table or more rows than the caller's "
+                "lists hold: that call changed nothing, and its rows were neither placed nor attended");
+  if (what == kMapBadEntry)
+    return fail(SHAINET_HIP_ERR_ARGUMENT,
+                "a map of new rows found a sequence out of range or named twice, or a length below 0: that call changed nothing, "
+                "and its rows were neither placed nor attended");
   if (what == 2)
     return fail(SHAINET_HIP_ERR_CAPACITY,
                 "a decode step found a sequence at the capacity of its cache or at the end of the context's "
@@ -519,6 +528,17 @@ int shainet_attn_run_biased(shainet_attn_ctx *c, shainet_kv_cache *kc, const flo
   st.tok_off[1] = new_tokens;
   Shape sh = shape_of(c, kc->cap);
   return run_attention(c, q, kc->k, kc->v, out, st, sh, new_tokens, c->scale, c->stream, nullptr, nullptr, &bias);
+}
+
+int shainet_attn_run_rows(shainet_attn_ctx *c, const float *q_rot, float *k, float *v, int cap, int start_pos, int new_tokens,
+                          float *out) {
+  SeqTable st;
+  memset(&st, 0, sizeof st);
+  st.n_seqs = 1;
+  st.start_pos[0] = start_pos;
+  st.n_new[0] = new_tokens;
+  st.tok_off[1] = new_tokens;
+  return run_attention(c, q_rot, k, v, out, st, shape_of(c, cap), new_tokens, c->scale, c->stream, nullptr);
 }
 
 extern "C" {

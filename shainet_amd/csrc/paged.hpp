@@ -1,0 +1,64 @@
+// Keys and values in pages: which page holds which rows (paged_map.hip), new rows into their slots (paged_append.hip),
+// attention of one new row per sequence over its pages (paged_attn.hip).  paged_cache.hip keeps the arrays and the C ABI.
+#pragma once
+#include <hip/hip_runtime.h>
+
+#include "attn_kernels.hpp"
+
+namespace shainet {
+
+constexpr int kPageF32 = 0, kPageBf16 = 1, kPageF16 = 2;
+constexpr int kMaxPagedSeqs = 4096;  // entries of a map, rows of an attention launch: their prefix sums lie in LDS
+inline int page_element_bytes(int dtype) { return dtype == kPageF32 ? 4 : 2; }
+
+// One layer's pages, [n_pages][KV][1 << shift][hd] for K and for V, and the table of all sequences.
+struct PagePool {
+  void *k, *v;
+  int dtype, KV, hd;
+  int n_pages, shift;     // rows per page: 1 << shift
+  const int *table;       // [n_seqs][seq_pages]
+  int n_seqs, seq_pages;
+};
+
+// A change of lengths: entry i is sequence ids[i], whose length changes by delta[i].
+struct MapArgs {
+  int n;
+  const int *ids, *delta;      // device; null: see `inlined`, else sequence i and one row
+  int inlined;                 // the two lists below instead, n <= kMaxSeqs
+  int id[kMaxSeqs], change[kMaxSeqs];
+  int *table, *lens, *free_pages, *n_free;
+  int n_seqs, seq_pages, n_pages, shift;
+  int *slots, *positions, *row_seqs;  // of the new rows in the entries' order; -1 from the last one to max_rows
+  int max_rows;
+  int *scratch;                // map_scratch_ints()
+  int *error;                  // device-writable: set to kMapNoRoom or kMapBadEntry where nothing was changed
+};
+constexpr int kMapNoRoom = 3, kMapBadEntry = 4;
+size_t map_scratch_ints();
+hipError_t launch_page_map(const MapArgs &a, hipStream_t stream);
+// every length 0, every page free, page 0 to be taken first
+hipError_t launch_page_reset(int *lens, int n_seqs, int *free_pages, int *n_free, int n_pages, hipStream_t stream);
+
+// bias -> QK-norm -> RoPE of `rows` rows, whose K and V parts go to slots[row] (page << shift | row in the page);
+// a.kc, a.vc are not used.  A row whose slot or position is out of range is left alone.
+hipError_t launch_paged_append(const PrepArgs &a, const PagePool &p, int H, const int *slots, const int *positions,
+                               int rope_positions, int rows, hipStream_t stream);
+
+// Attention of row r of q ([rows][H * hd], rows q_stride floats apart) over the first positions[r] + 1 rows of sequence
+// row_seqs[r].  A row with row_seqs < 0 is left alone; one with positions < 0 gets zeros.
+struct PagedAttendArgs {
+  const float *q;
+  float *out;
+  long long q_stride, out_stride;
+  const int *row_seqs, *positions;
+  int rows, H;
+  float scale;
+  void *workspace;             // paged_attend_workspace() bytes, its first kPagedTickets words zero, which a launch leaves so
+};
+size_t paged_attend_workspace(int hd);
+hipError_t launch_paged_attend(const PagedAttendArgs &a, const PagePool &p, hipStream_t stream);
+
+// The first n rows of a sequence, as floats, into [KV][cap][hd] arrays.
+hipError_t launch_page_gather(const PagePool &p, int seq, int pos0, int n, int cap, float *k, float *v, hipStream_t stream);
+
+}  // namespace shainet

@@ -1,0 +1,566 @@
+// shainet_paged_cache: keys and values in pages, the tables that say which sequence holds which page, and the calls of an
+// AttnContext over them (declared in include/shainet_hip_attn.h).
+#include <hip/hip_runtime.h>
+#include <stdarg.h>
+#include <stdio.h>
+#include <string.h>
+
+#include <new>
+#include <vector>
+
+#include "../../include/shainet_hip_attn.h"
+#include "attn_context.hpp"
+#include "attn_kernels.hpp"
+#include "llama_internal.hpp"
+#include "paged.hpp"
+
+using namespace shainet;
+
+void shainet_hip_set_error(int code, const char *msg);
+
+struct shainet_paged_cache {
+  shainet_attn_ctx *ctx;
+  int device;
+  int layers, KV, hd, dtype, n_pages, shift, n_seqs, seq_pages;
+  size_t layer_bytes;  // of K, and of V
+  char *k = nullptr, *v = nullptr;
+  int *table = nullptr, *lens = nullptr, *free_pages = nullptr, *n_free = nullptr;
+  int *pin = nullptr;      // [n_seqs + 1] on its way from the device
+  int *scratch = nullptr;  // map_scratch_ints()
+  void *workspace = nullptr;
+  // steps: allocated with the cache, so that a step allocates nothing
+  int *step_slots = nullptr, *step_positions = nullptr, *step_seqs = nullptr;  // [n_seqs]
+  DevBuf step_q;           // [n_seqs, H hd] of the owner's context; other contexts have at most as many heads
+  int step_rows = 0;       // of the last step that mapped rows; 0: none yet
+  // forward calls: grow on demand
+  DevBuf rows;             // three lists of ints
+  DevBuf gathered;
+  std::vector<int> len;    // per sequence, while the host knows them
+  int free_count;
+  bool lengths_on_device = false;
+  std::vector<int> last_ids, last_new, last_start;  // of the last forward call for layer 0
+};
+
+namespace {
+
+int fail(int code, const char *fmt, ...) {
+  char text[512];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(text, sizeof text, fmt, ap);
+  va_end(ap);
+  shainet_hip_set_error(code, text);
+  return code;
+}
+
+int hip_fail(hipError_t e, const char *what) {
+  (void)hipGetLastError();
+  return fail(e == hipErrorOutOfMemory ? SHAINET_HIP_ERR_ALLOC : SHAINET_HIP_ERR_RUNTIME, "%s: %s", what, hipGetErrorString(e));
+}
+
+#define HIP_TRY(expr)                                 \
+  do {                                                \
+    hipError_t e_ = (expr);                           \
+    if (e_ != hipSuccess) return hip_fail(e_, #expr); \
+  } while (0)
+
+int pages_of(const shainet_paged_cache *pc, long long rows) { return (int)((rows + (1 << pc->shift) - 1) >> pc->shift); }
+long long reach_of(const shainet_paged_cache *pc) { return (long long)pc->seq_pages << pc->shift; }
+
+PagePool pool_of(const shainet_paged_cache *pc, int layer) {
+  PagePool p;
+  p.k = pc->k + (size_t)layer * pc->layer_bytes;
+  p.v = pc->v + (size_t)layer * pc->layer_bytes;
+  p.dtype = pc->dtype;
+  p.KV = pc->KV;
+  p.hd = pc->hd;
+  p.n_pages = pc->n_pages;
+  p.shift = pc->shift;
+  p.table = pc->table;
+  p.n_seqs = pc->n_seqs;
+  p.seq_pages = pc->seq_pages;
+  return p;
+}
+
+// What every call that launches something asks first.
+int check_device(const shainet_paged_cache *pc) {
+  int device = -1;
+  HIP_TRY(hipGetDevice(&device));
+  if (device != pc->device)
+    return fail(SHAINET_HIP_ERR_ARGUMENT, "the cache is on device %d, the current device is %d", pc->device, device);
+  return SHAINET_HIP_OK;
+}
+
+int check_pair(const shainet_attn_ctx *c, const shainet_paged_cache *pc, int layer) {
+  if (!c || !pc || c->KV != pc->KV || c->hd != pc->hd || c->v_hd != pc->hd || c->window || c->rope_fp64)
+    return fail(SHAINET_HIP_ERR_ARGUMENT, "context and cache do not belong together");
+  if (c->H > pc->ctx->H) return fail(SHAINET_HIP_ERR_ARGUMENT, "the context has more query heads than the one the cache was made with");
+  if (c->stream != pc->ctx->stream)
+    return fail(SHAINET_HIP_ERR_ARGUMENT, "contexts that share a cache work on one stream: shainet_attn_set_stream");
+  if (layer < 0 || layer >= pc->layers) return fail(SHAINET_HIP_ERR_ARGUMENT, "layer must be in 0..%d", pc->layers - 1);
+  return check_device(pc);
+}
+
+int refuse_unknown_lengths(const shainet_paged_cache *pc, const char *what) {
+  if (!pc->lengths_on_device) return SHAINET_HIP_OK;
+  return fail(SHAINET_HIP_ERR_ARGUMENT, "%s: the lengths were changed on the device; call shainet_paged_cache_lengths_from_device first", what);
+}
+
+MapArgs map_of(const shainet_paged_cache *pc) {
+  MapArgs a;
+  memset(&a, 0, sizeof a);
+  a.table = pc->table;
+  a.lens = pc->lens;
+  a.free_pages = pc->free_pages;
+  a.n_free = pc->n_free;
+  a.n_seqs = pc->n_seqs;
+  a.seq_pages = pc->seq_pages;
+  a.n_pages = pc->n_pages;
+  a.shift = pc->shift;
+  a.scratch = pc->scratch;
+  a.error = pc->ctx->error;
+  return a;
+}
+
+// The lengths of up to kMaxSeqs sequences that the host knows change by `change`; rows (nullable): three lists of max_rows.
+int map_listed(shainet_paged_cache *pc, const int *ids, const int *change, int n, int *rows, int max_rows) {
+  MapArgs a = map_of(pc);
+  a.n = n;
+  a.inlined = 1;
+  for (int i = 0; i < n; ++i) {
+    a.id[i] = ids[i];
+    a.change[i] = change[i];
+  }
+  a.max_rows = max_rows;
+  if (rows) {
+    a.slots = rows;
+    a.positions = rows + max_rows;
+    a.row_seqs = rows + 2 * (size_t)max_rows;
+  }
+  const hipError_t e = launch_page_map(a, pc->ctx->stream);
+  return e == hipSuccess ? SHAINET_HIP_OK : hip_fail(e, "map launch");
+}
+
+// The cos/sin table reaches as far as a sequence can: which positions a map holds is known to the device only.
+int reach_table(shainet_attn_ctx *c, const shainet_paged_cache *pc) {
+  if (c->rope_positions >= reach_of(pc)) return SHAINET_HIP_OK;
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  if (c->stream) HIP_TRY(hipStreamIsCapturing(c->stream, &status));
+  if (status != hipStreamCaptureStatusNone)
+    return fail(SHAINET_HIP_ERR_ARGUMENT, "the context's cos/sin table must be extended to %lld positions, which cannot be recorded: create the context "
+                "with that many, or place rows once before recording", reach_of(pc));
+  return ensure_rope_table(c, (int)reach_of(pc));
+}
+
+PrepArgs prep_of(const shainet_attn_ctx *c, const float *q, long long q_stride, const float *k, long long k_stride, const float *v,
+                 long long v_stride, float *q_rot) {
+  PrepArgs pa;
+  memset(&pa, 0, sizeof pa);
+  pa.q = q;
+  pa.k = k;
+  pa.v = v;
+  pa.q_stride = q_stride;
+  pa.k_stride = k_stride;
+  pa.v_stride = v_stride;
+  pa.b_q = c->d_bq;
+  pa.b_k = c->d_bk;
+  pa.b_v = c->d_bv;
+  pa.q_norm = c->d_q_norm;
+  pa.k_norm = c->d_k_norm;
+  pa.eps = c->eps;
+  pa.rope_tab = c->d_rope;
+  pa.q_rot = q_rot;
+  return pa;
+}
+
+int append(shainet_attn_ctx *c, shainet_paged_cache *pc, int layer, const PrepArgs &pa, const int *slots, const int *positions,
+           int rows) {
+  const hipError_t e = launch_paged_append(pa, pool_of(pc, layer), c->H, slots, positions, c->rope_positions, rows, c->stream);
+  return e == hipSuccess ? SHAINET_HIP_OK : hip_fail(e, "append launch");
+}
+
+int attend(shainet_attn_ctx *c, shainet_paged_cache *pc, int layer, const int *row_seqs, const int *positions, int rows,
+           const float *q, long long q_stride, float *out, long long out_stride) {
+  PagedAttendArgs a;
+  a.q = q;
+  a.out = out;
+  a.q_stride = q_stride;
+  a.out_stride = out_stride;
+  a.row_seqs = row_seqs;
+  a.positions = positions;
+  a.rows = rows;
+  a.H = c->H;
+  a.scale = c->scale;
+  a.workspace = pc->workspace;
+  const hipError_t e = launch_paged_attend(a, pool_of(pc, layer), c->stream);
+  return e == hipSuccess ? SHAINET_HIP_OK : hip_fail(e, "attention launch");
+}
+
+// New rows of a sequence up to this many read the pages themselves, one by one; more are gathered for first, once for all of them.
+constexpr int kRowsFromPages = 4;
+
+}  // namespace
+
+extern "C" {
+
+int shainet_paged_cache_create(shainet_paged_cache **out, shainet_attn_ctx *ctx, int layers, int n_pages, int page_rows, int n_seqs,
+                               int seq_pages, int dtype) {
+  if (!out) return fail(SHAINET_HIP_ERR_ARGUMENT, "out is null");
+  *out = nullptr;
+  if (!ctx) return fail(SHAINET_HIP_ERR_ARGUMENT, "ctx is null");
+  if (ctx->v_hd != ctx->hd || ctx->window || ctx->rope_fp64 || (ctx->hd & 7))
+    return fail(SHAINET_HIP_ERR_ARGUMENT, "a cache in pages needs grouped-query attention with rotation and a head_dim that is a multiple of 8 up to 256");
+  if (page_rows < 8 || page_rows > 1024 || (page_rows & (page_rows - 1)))
+    return fail(SHAINET_HIP_ERR_ARGUMENT, "page_rows must be a power of two in 8..1024");
+  if (dtype != SHAINET_HIP_PAGE_F32 && dtype != SHAINET_HIP_PAGE_BF16 && dtype != SHAINET_HIP_PAGE_F16)
+    return fail(SHAINET_HIP_ERR_ARGUMENT, "dtype must be one of SHAINET_HIP_PAGE_F32, _BF16 and _F16");
+  if (n_seqs < 1 || n_seqs > SHAINET_HIP_MAX_PAGED_SEQS)
+    return fail(SHAINET_HIP_ERR_ARGUMENT, "n_seqs must be in 1..%d", SHAINET_HIP_MAX_PAGED_SEQS);
+  if (layers < 1 || n_pages < 1 || seq_pages < 1 || (long long)n_pages * page_rows > 0x7fffffffLL ||
+      (long long)seq_pages * page_rows > 0x3fffffffLL || (long long)n_seqs * seq_pages > 0x7fffffffLL)
+    return fail(SHAINET_HIP_ERR_ARGUMENT, "invalid cache geometry: slots and table entries are 32-bit numbers, positions 30-bit ones");
+  shainet_paged_cache *pc = new (std::nothrow) shainet_paged_cache();
+  if (!pc) return fail(SHAINET_HIP_ERR_ALLOC, "out of host memory");
+  pc->ctx = ctx;
+  pc->layers = layers;
+  pc->KV = ctx->KV;
+  pc->hd = ctx->hd;
+  pc->dtype = dtype;
+  pc->n_pages = n_pages;
+  pc->shift = __builtin_ctz((unsigned)page_rows);
+  pc->n_seqs = n_seqs;
+  pc->seq_pages = seq_pages;
+  pc->free_count = n_pages;
+  pc->layer_bytes = (size_t)n_pages * ctx->KV * page_rows * ctx->hd * page_element_bytes(dtype);
+  int rc = SHAINET_HIP_OK;
+  try {
+    pc->len.assign(n_seqs, 0);
+  } catch (const std::bad_alloc &) {
+    rc = fail(SHAINET_HIP_ERR_ALLOC, "out of host memory");
+  }
+  const size_t pool = pc->layer_bytes * layers, table = (size_t)n_seqs * seq_pages, ws = paged_attend_workspace(ctx->hd);
+  hipError_t e = rc ? hipErrorOutOfMemory : hipGetDevice(&pc->device);
+  if (e == hipSuccess) e = hipMalloc((void **)&pc->k, pool);
+  if (e == hipSuccess) e = hipMalloc((void **)&pc->v, pool);
+  if (e == hipSuccess) e = hipMalloc((void **)&pc->table, table * sizeof(int));
+  if (e == hipSuccess) e = hipMalloc((void **)&pc->lens, n_seqs * sizeof(int));
+  if (e == hipSuccess) e = hipMalloc((void **)&pc->free_pages, (size_t)n_pages * sizeof(int));
+  if (e == hipSuccess) e = hipMalloc((void **)&pc->n_free, sizeof(int));
+  if (e == hipSuccess) e = hipHostMalloc((void **)&pc->pin, (n_seqs + 1) * sizeof(int), hipHostMallocDefault);
+  if (e == hipSuccess) e = hipMalloc((void **)&pc->scratch, map_scratch_ints() * sizeof(int));
+  if (e == hipSuccess) e = hipMalloc(&pc->workspace, ws);
+  if (e == hipSuccess) e = hipMalloc((void **)&pc->step_slots, n_seqs * sizeof(int));
+  if (e == hipSuccess) e = hipMalloc((void **)&pc->step_positions, n_seqs * sizeof(int));
+  if (e == hipSuccess) e = hipMalloc((void **)&pc->step_seqs, n_seqs * sizeof(int));
+  // (rows never written hold zeros; on the stream that uses them, and waited for)
+  if (e == hipSuccess) e = hipMemsetAsync(pc->k, 0, pool, ctx->stream);
+  if (e == hipSuccess) e = hipMemsetAsync(pc->v, 0, pool, ctx->stream);
+  if (e == hipSuccess) e = hipMemsetAsync(pc->table, 0xff, table * sizeof(int), ctx->stream);
+  if (e == hipSuccess) e = hipMemsetAsync(pc->workspace, 0, ws, ctx->stream);
+  if (e == hipSuccess) e = launch_page_reset(pc->lens, n_seqs, pc->free_pages, pc->n_free, n_pages, ctx->stream);
+  if (e == hipSuccess) e = hipStreamSynchronize(ctx->stream);
+  if (e != hipSuccess && !rc) rc = hip_fail(e, "allocation of a cache in pages");
+  if (!rc) rc = pc->step_q.reserve((size_t)n_seqs * ctx->H * ctx->hd);
+  if (rc) {
+    shainet_paged_cache_destroy(pc);
+    return rc;
+  }
+  *out = pc;
+  return SHAINET_HIP_OK;
+}
+
+int shainet_paged_cache_destroy(shainet_paged_cache *pc) {
+  if (!pc) return SHAINET_HIP_OK;
+  (void)hipStreamSynchronize(pc->ctx->stream);
+  for (void *p : {(void *)pc->k, (void *)pc->v, (void *)pc->table, (void *)pc->lens, (void *)pc->free_pages, (void *)pc->n_free,
+                  (void *)pc->scratch, pc->workspace, (void *)pc->step_slots, (void *)pc->step_positions, (void *)pc->step_seqs})
+    if (p) (void)hipFree(p);
+  if (pc->pin) (void)hipHostFree(pc->pin);
+  for (DevBuf *b : {&pc->step_q, &pc->rows, &pc->gathered}) b->release();
+  delete pc;
+  return SHAINET_HIP_OK;
+}
+
+int shainet_paged_cache_arrays(shainet_paged_cache *pc, int layer, void **k, void **v, int **table, int **lens, int **free_pages,
+                               int **n_free) {
+  if (!pc || layer < 0 || layer >= pc->layers) return fail(SHAINET_HIP_ERR_ARGUMENT, "invalid cache or layer");
+  const PagePool p = pool_of(pc, layer);
+  if (k) *k = p.k;
+  if (v) *v = p.v;
+  if (table) *table = pc->table;
+  if (lens) *lens = pc->lens;
+  if (free_pages) *free_pages = pc->free_pages;
+  if (n_free) *n_free = pc->n_free;
+  return SHAINET_HIP_OK;
+}
+
+int shainet_paged_cache_map_rows(shainet_paged_cache *pc, const int *seq_ids, const int *delta, int n, int *slots, int *positions,
+                                 int *row_seqs, int max_rows) {
+  if (!pc || !delta) return fail(SHAINET_HIP_ERR_ARGUMENT, "null argument");
+  if (n < 1 || n > pc->n_seqs) return fail(SHAINET_HIP_ERR_ARGUMENT, "n must be in 1..%d", pc->n_seqs);
+  if (max_rows < 0) return fail(SHAINET_HIP_ERR_ARGUMENT, "max_rows must not be negative");
+  if (max_rows && (!slots || !positions || !row_seqs)) return fail(SHAINET_HIP_ERR_ARGUMENT, "null argument");
+  if (int rc = check_device(pc)) return rc;
+  MapArgs a = map_of(pc);
+  a.n = n;
+  a.ids = seq_ids;
+  a.delta = delta;
+  a.slots = slots;
+  a.positions = positions;
+  a.row_seqs = row_seqs;
+  a.max_rows = max_rows;
+  const hipError_t e = launch_page_map(a, pc->ctx->stream);
+  if (e != hipSuccess) return hip_fail(e, "map launch");
+  pc->lengths_on_device = true;
+  return SHAINET_HIP_OK;
+}
+
+int shainet_paged_cache_lengths_from_device(shainet_paged_cache *pc) {
+  if (!pc) return fail(SHAINET_HIP_ERR_ARGUMENT, "cache is null");
+  if (int rc = check_device(pc)) return rc;
+  HIP_TRY(hipMemcpyAsync(pc->pin, pc->lens, pc->n_seqs * sizeof(int), hipMemcpyDeviceToHost, pc->ctx->stream));
+  HIP_TRY(hipMemcpyAsync(pc->pin + pc->n_seqs, pc->n_free, sizeof(int), hipMemcpyDeviceToHost, pc->ctx->stream));
+  HIP_TRY(hipStreamSynchronize(pc->ctx->stream));
+  for (int s = 0; s < pc->n_seqs; ++s)
+    if (pc->pin[s] < 0 || pc->pin[s] > reach_of(pc))
+      return fail(SHAINET_HIP_ERR_RUNTIME, "the device holds length %d for sequence %d", pc->pin[s], s);
+  if (pc->pin[pc->n_seqs] < 0 || pc->pin[pc->n_seqs] > pc->n_pages)
+    return fail(SHAINET_HIP_ERR_RUNTIME, "the device holds %d free pages of %d", pc->pin[pc->n_seqs], pc->n_pages);
+  memcpy(pc->len.data(), pc->pin, pc->n_seqs * sizeof(int));
+  pc->free_count = pc->pin[pc->n_seqs];
+  pc->lengths_on_device = false;
+  return check_error_word(pc->ctx->error);
+}
+
+int shainet_paged_cache_len(const shainet_paged_cache *pc, int seq) {
+  if (!pc || seq < 0 || seq >= pc->n_seqs || refuse_unknown_lengths(pc, "shainet_paged_cache_len")) return -1;
+  return pc->len[seq];
+}
+
+int shainet_paged_cache_free_pages(const shainet_paged_cache *pc) {
+  if (!pc || refuse_unknown_lengths(pc, "shainet_paged_cache_free_pages")) return -1;
+  return pc->free_count;
+}
+
+int shainet_paged_cache_truncate(shainet_paged_cache *pc, int seq, int len) {
+  if (!pc || seq < 0 || seq >= pc->n_seqs) return fail(SHAINET_HIP_ERR_ARGUMENT, "invalid sequence");
+  if (int rc = refuse_unknown_lengths(pc, "shainet_paged_cache_truncate")) return rc;
+  if (len < 0 || len > pc->len[seq]) return fail(SHAINET_HIP_ERR_ARGUMENT, "truncate to %d outside 0..%d", len, pc->len[seq]);
+  if (int rc = check_device(pc)) return rc;
+  const int change = len - pc->len[seq];
+  if (change == 0) return SHAINET_HIP_OK;
+  if (int rc = map_listed(pc, &seq, &change, 1, nullptr, 0)) return rc;
+  pc->free_count += pages_of(pc, pc->len[seq]) - pages_of(pc, len);
+  pc->len[seq] = len;
+  pc->last_ids.clear();
+  return SHAINET_HIP_OK;
+}
+
+int shainet_paged_cache_clear(shainet_paged_cache *pc, int seq) {
+  if (!pc || seq >= pc->n_seqs) return fail(SHAINET_HIP_ERR_ARGUMENT, "invalid sequence");
+  if (seq >= 0) return shainet_paged_cache_truncate(pc, seq, 0);
+  if (int rc = check_device(pc)) return rc;
+  const hipError_t e = launch_page_reset(pc->lens, pc->n_seqs, pc->free_pages, pc->n_free, pc->n_pages, pc->ctx->stream);
+  if (e != hipSuccess) return hip_fail(e, "reset launch");
+  pc->len.assign(pc->n_seqs, 0);
+  pc->free_count = pc->n_pages;
+  pc->lengths_on_device = false;
+  pc->last_ids.clear();
+  pc->step_rows = 0;
+  return SHAINET_HIP_OK;
+}
+
+int shainet_paged_cache_read(shainet_paged_cache *pc, int layer, int seq, int kv_head, int pos0, int n, float *k_out, float *v_out) {
+  if (!pc || layer < 0 || layer >= pc->layers || seq < 0 || seq >= pc->n_seqs || kv_head < 0 || kv_head >= pc->KV || pos0 < 0 || n < 0)
+    return fail(SHAINET_HIP_ERR_ARGUMENT, "invalid read arguments");
+  if (int rc = refuse_unknown_lengths(pc, "shainet_paged_cache_read")) return rc;
+  if ((long long)pos0 + n > pc->len[seq]) return fail(SHAINET_HIP_ERR_ARGUMENT, "rows %d..%lld of a sequence of %d", pos0, (long long)pos0 + n - 1, pc->len[seq]);
+  if (n == 0) return SHAINET_HIP_OK;
+  if (int rc = check_device(pc)) return rc;
+  const size_t each = (size_t)pc->KV * n * pc->hd;
+  if (int rc = pc->gathered.reserve(2 * each)) return rc;
+  float *k = pc->gathered.p, *v = k + each;
+  const hipError_t e = launch_page_gather(pool_of(pc, layer), seq, pos0, n, n, k, v, pc->ctx->stream);
+  if (e != hipSuccess) return hip_fail(e, "gather launch");
+  HIP_TRY(hipStreamSynchronize(pc->ctx->stream));
+  const size_t first = (size_t)kv_head * n * pc->hd, bytes = (size_t)n * pc->hd * sizeof(float);
+  if (k_out) HIP_TRY(hipMemcpy(k_out, k + first, bytes, hipMemcpyDeviceToHost));
+  if (v_out) HIP_TRY(hipMemcpy(v_out, v + first, bytes, hipMemcpyDeviceToHost));
+  return SHAINET_HIP_OK;
+}
+
+int shainet_attn_append_paged(shainet_attn_ctx *c, shainet_paged_cache *pc, int layer, const int *slots, const int *positions, int rows,
+                              const float *q, long long q_stride, const float *k, long long k_stride, const float *v,
+                              long long v_stride, float *q_rot) {
+  if (int rc = check_pair(c, pc, layer)) return rc;
+  if (!slots || !positions || !q || !k || !v || !q_rot) return fail(SHAINET_HIP_ERR_ARGUMENT, "null argument");
+  if (rows < 1 || rows > 0x3fffffff / (c->H + 2 * c->KV)) return fail(SHAINET_HIP_ERR_ARGUMENT, "rows must be in 1..%d", 0x3fffffff / (c->H + 2 * c->KV));
+  if (q_stride < (long long)c->H * c->hd || k_stride < (long long)c->KV * c->hd || v_stride < (long long)c->KV * c->hd)
+    return fail(SHAINET_HIP_ERR_ARGUMENT, "row strides must be at least the row widths %d and %d", c->H * c->hd, c->KV * c->hd);
+  if (int rc = reach_table(c, pc)) return rc;
+  return append(c, pc, layer, prep_of(c, q, q_stride, k, k_stride, v, v_stride, q_rot), slots, positions, rows);
+}
+
+int shainet_attn_attend_paged(shainet_attn_ctx *c, shainet_paged_cache *pc, int layer, const int *row_seqs, const int *positions,
+                              int rows, const float *q_rot, long long q_stride, float *out, long long out_stride) {
+  if (int rc = check_pair(c, pc, layer)) return rc;
+  if (!row_seqs || !positions || !q_rot || !out) return fail(SHAINET_HIP_ERR_ARGUMENT, "null argument");
+  if (rows < 1 || rows > SHAINET_HIP_MAX_PAGED_SEQS)
+    return fail(SHAINET_HIP_ERR_ARGUMENT, "rows must be in 1..%d", SHAINET_HIP_MAX_PAGED_SEQS);
+  if (q_stride < (long long)c->H * c->hd || out_stride < (long long)c->H * c->hd)
+    return fail(SHAINET_HIP_ERR_ARGUMENT, "row strides must be at least the row width %d", c->H * c->hd);
+  return attend(c, pc, layer, row_seqs, positions, rows, q_rot, q_stride, out, out_stride);
+}
+
+int shainet_attn_step_paged(shainet_attn_ctx *c, shainet_paged_cache *pc, int layer, const int *seq_ids, int n, const float *q,
+                            const float *k, const float *v, float *out) {
+  if (int rc = check_pair(c, pc, layer)) return rc;
+  if (!q || !k || !v || !out) return fail(SHAINET_HIP_ERR_ARGUMENT, "null argument");
+  if (n < 1 || n > pc->n_seqs) return fail(SHAINET_HIP_ERR_ARGUMENT, "n must be in 1..%d", pc->n_seqs);
+  if (layer > 0 && n != pc->step_rows)
+    return fail(SHAINET_HIP_ERR_ARGUMENT, "layer %d of a step of %d rows: layer 0 mapped %d", layer, n, pc->step_rows);
+  if (int rc = reach_table(c, pc)) return rc;
+  if (layer == 0) {
+    MapArgs a = map_of(pc);
+    a.n = n;
+    a.ids = seq_ids;
+    a.slots = pc->step_slots;
+    a.positions = pc->step_positions;
+    a.row_seqs = pc->step_seqs;
+    a.max_rows = n;
+    const hipError_t e = launch_page_map(a, c->stream);
+    if (e != hipSuccess) return hip_fail(e, "map launch");
+    pc->lengths_on_device = true;
+    pc->step_rows = n;
+    pc->last_ids.clear();
+  }
+  const long long q_dim = (long long)c->H * c->hd, kv_dim = (long long)c->KV * c->hd;
+  float *q_rot = pc->step_q.p;
+  if (int rc = append(c, pc, layer, prep_of(c, q, q_dim, k, kv_dim, v, kv_dim, q_rot), pc->step_slots, pc->step_positions, n)) return rc;
+  return attend(c, pc, layer, pc->step_seqs, pc->step_positions, n, q_rot, q_dim, out, q_dim);
+}
+
+int shainet_attn_forward_paged(shainet_attn_ctx *c, shainet_paged_cache *pc, int layer, const int *seq_ids, const int *new_tokens,
+                               int n_seqs, const float *q, const float *k, const float *v, float *out, int mem) {
+  if (int rc = check_pair(c, pc, layer)) return rc;
+  if (!new_tokens || !q || !k || !v || !out) return fail(SHAINET_HIP_ERR_ARGUMENT, "null argument");
+  if (mem != SHAINET_HIP_MEM_HOST && mem != SHAINET_HIP_MEM_DEVICE)
+    return fail(SHAINET_HIP_ERR_ARGUMENT, "mem must be SHAINET_HIP_MEM_HOST or SHAINET_HIP_MEM_DEVICE");
+  if (n_seqs < 1 || n_seqs > SHAINET_HIP_MAX_BATCH) return fail(SHAINET_HIP_ERR_ARGUMENT, "n_seqs must be in 1..%d", SHAINET_HIP_MAX_BATCH);
+  if (int rc = refuse_unknown_lengths(pc, "shainet_attn_forward_paged")) return rc;
+  int ids[kMaxSeqs], start[kMaxSeqs], change[kMaxSeqs], longest = 0;
+  long long total = 0, pages = 0;
+  for (int s = 0; s < n_seqs; ++s) {
+    const int id = ids[s] = seq_ids ? seq_ids[s] : s, more = change[s] = new_tokens[s];
+    if (id < 0 || id >= pc->n_seqs) return fail(SHAINET_HIP_ERR_ARGUMENT, "sequence id %d out of range", id);
+    for (int t = 0; t < s; ++t)
+      if (ids[t] == id) return fail(SHAINET_HIP_ERR_ARGUMENT, "sequence id %d appears twice", id);
+    if (more < 1) return fail(SHAINET_HIP_ERR_ARGUMENT, "new_tokens must be positive");
+    // (layers behind the first: the rows are counted already)
+    start[s] = layer == 0 ? pc->len[id] : pc->len[id] - more;
+    if ((long long)start[s] + more > reach_of(pc))
+      return fail(SHAINET_HIP_ERR_CAPACITY, "sequence %d: %d cached + %d new rows exceed the %lld of its table", id, start[s], more, reach_of(pc));
+    pages += pages_of(pc, (long long)start[s] + more) - pages_of(pc, start[s]);
+    total += more;
+    if (total > 0x3fffffff / (c->H + 2 * c->KV)) return fail(SHAINET_HIP_ERR_ARGUMENT, "too many rows in one call");
+    if (more > kRowsFromPages && start[s] + more > longest) longest = start[s] + more;
+  }
+  if (layer == 0 && pages > pc->free_count)
+    return fail(SHAINET_HIP_ERR_CAPACITY, "%lld pages wanted, %d free", pages, pc->free_count);
+  if (layer > 0 && ((int)pc->last_ids.size() != n_seqs || memcmp(pc->last_ids.data(), ids, n_seqs * sizeof(int)) ||
+                    memcmp(pc->last_new.data(), change, n_seqs * sizeof(int))))
+    return fail(SHAINET_HIP_ERR_ARGUMENT, "layer %d: other rows than layer 0 of this cache had last", layer);
+  const int rows = (int)total;
+  const size_t q_floats = (size_t)rows * c->H * c->hd, kv_floats = (size_t)rows * c->KV * c->hd, gathered = (size_t)c->KV * longest * c->hd;
+  int rc = reach_table(c, pc);
+  if (!rc) rc = c->q_rot.reserve(q_floats);
+  if (!rc && layer == 0) rc = pc->rows.reserve(3 * (size_t)rows);
+  if (!rc && longest) rc = pc->gathered.reserve(2 * gathered);
+  const float *dq = q, *dk = k, *dv = v;
+  float *dout = out;
+  if (!rc && mem == SHAINET_HIP_MEM_HOST) {
+    (void)((rc = c->in_q.reserve(q_floats)) || (rc = c->in_k.reserve(kv_floats)) || (rc = c->in_v.reserve(kv_floats)) ||
+           (rc = c->out.reserve(q_floats)) || (rc = c->pin_in.reserve(q_floats + 2 * kv_floats)) || (rc = c->pin_out.reserve(q_floats)));
+    if (rc) return rc;
+    float *pq = c->pin_in.p, *pk = pq + q_floats, *pv = pk + kv_floats;
+    memcpy(pq, q, q_floats * sizeof(float));
+    memcpy(pk, k, kv_floats * sizeof(float));
+    memcpy(pv, v, kv_floats * sizeof(float));
+    hipError_t ce = hipMemcpyAsync(c->in_q.p, pq, q_floats * sizeof(float), hipMemcpyHostToDevice, c->stream);
+    if (ce == hipSuccess) ce = hipMemcpyAsync(c->in_k.p, pk, kv_floats * sizeof(float), hipMemcpyHostToDevice, c->stream);
+    if (ce == hipSuccess) ce = hipMemcpyAsync(c->in_v.p, pv, kv_floats * sizeof(float), hipMemcpyHostToDevice, c->stream);
+    if (ce != hipSuccess) {
+      (void)hipStreamSynchronize(c->stream);  // a copy already queued may still read the staging buffer
+      return hip_fail(ce, "hipMemcpyAsync(q, k, v)");
+    }
+    dq = c->in_q.p;
+    dk = c->in_k.p;
+    dv = c->in_v.p;
+    dout = c->out.p;
+  }
+  if (rc) return rc;
+  int *lists = (int *)pc->rows.p;
+  const int *slots = lists, *positions = lists + rows, *row_seqs = lists + 2 * (size_t)rows;
+  if (layer == 0) {
+    try {
+      pc->last_ids.assign(ids, ids + n_seqs);
+      pc->last_new.assign(change, change + n_seqs);
+    } catch (const std::bad_alloc &) {
+      pc->last_ids.clear();
+      rc = fail(SHAINET_HIP_ERR_ALLOC, "out of host memory");
+    }
+    if (!rc) rc = map_listed(pc, ids, change, n_seqs, lists, rows);
+    if (rc) {
+      if (mem == SHAINET_HIP_MEM_HOST) (void)hipStreamSynchronize(c->stream);
+      return rc;
+    }
+  }
+  const long long q_dim = (long long)c->H * c->hd, kv_dim = (long long)c->KV * c->hd;
+  rc = append(c, pc, layer, prep_of(c, dq, q_dim, dk, kv_dim, dv, kv_dim, c->q_rot.p), slots, positions, rows);
+  // entries of a few rows each go together, from row `done` on; one of many by itself
+  int at = 0, done = 0;
+  for (int s = 0; s <= n_seqs && !rc; ++s) {
+    const bool many = s < n_seqs && change[s] > kRowsFromPages;
+    while ((many || s == n_seqs) && done < at && !rc) {
+      const int some = at - done < kMaxPagedSeqs ? at - done : kMaxPagedSeqs;
+      rc = attend(c, pc, layer, row_seqs + done, positions + done, some, c->q_rot.p + done * q_dim, q_dim, dout + done * q_dim, q_dim);
+      done += some;
+    }
+    if (s == n_seqs || rc) break;
+    if (many) {
+      const int cap = start[s] + change[s];
+      float *gk = pc->gathered.p, *gv = gk + gathered;
+      const hipError_t e = launch_page_gather(pool_of(pc, layer), ids[s], 0, cap, cap, gk, gv, c->stream);
+      rc = e == hipSuccess ? shainet_attn_run_rows(c, c->q_rot.p + at * q_dim, gk, gv, cap, start[s], change[s], dout + at * q_dim)
+                           : hip_fail(e, "gather launch");
+      done = at + change[s];
+    }
+    at += change[s];
+  }
+  if (rc) {
+    if (layer == 0) {  // the rows leave again: the call did not happen
+      for (int s = 0; s < n_seqs; ++s) change[s] = -change[s];
+      (void)map_listed(pc, ids, change, n_seqs, nullptr, 0);
+      pc->last_ids.clear();
+    }
+    if (mem == SHAINET_HIP_MEM_HOST) (void)hipStreamSynchronize(c->stream);
+    return rc;
+  }
+  if (layer == 0) {
+    for (int s = 0; s < n_seqs; ++s) pc->len[ids[s]] += change[s];
+    pc->free_count -= (int)pages;
+    pc->step_rows = 0;
+  }
+  c->last_rows = rows;
+  if (mem == SHAINET_HIP_MEM_HOST) {
+    const hipError_t ce = hipMemcpyAsync(c->pin_out.p, dout, q_floats * sizeof(float), hipMemcpyDeviceToHost, c->stream);
+    const hipError_t se = hipStreamSynchronize(c->stream);  // also when the copy could not be queued
+    if (ce != hipSuccess) return hip_fail(ce, "hipMemcpyAsync(out)");
+    if (se != hipSuccess) return hip_fail(se, "hipStreamSynchronize");
+    memcpy(out, c->pin_out.p, q_floats * sizeof(float));
+    return check_error_word(c->error);
+  }
+  return SHAINET_HIP_OK;
+}
+
+}  // extern "C"

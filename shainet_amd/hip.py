@@ -78,6 +78,25 @@ _SIGNATURES = {
     "shainet_kv_cache_lengths_from_device": (C.c_int, [C.c_void_p]),
     "shainet_attn_decode_step": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p,
                                            C.c_void_p]),
+    "shainet_paged_cache_create": (C.c_int, [C.POINTER(C.c_void_p), C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int]),
+    "shainet_paged_cache_destroy": (C.c_int, [C.c_void_p]),
+    "shainet_paged_cache_arrays": (C.c_int, [C.c_void_p, C.c_int] + [C.POINTER(C.c_void_p)] * 6),
+    "shainet_paged_cache_map_rows": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p,
+                                               C.c_int]),
+    "shainet_paged_cache_lengths_from_device": (C.c_int, [C.c_void_p]),
+    "shainet_paged_cache_len": (C.c_int, [C.c_void_p, C.c_int]),
+    "shainet_paged_cache_free_pages": (C.c_int, [C.c_void_p]),
+    "shainet_paged_cache_truncate": (C.c_int, [C.c_void_p, C.c_int, C.c_int]),
+    "shainet_paged_cache_clear": (C.c_int, [C.c_void_p, C.c_int]),
+    "shainet_paged_cache_read": (C.c_int, [C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, _f32p, _f32p]),
+    "shainet_attn_append_paged": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p,
+                                            C.c_longlong, C.c_void_p, C.c_longlong, C.c_void_p, C.c_longlong, C.c_void_p]),
+    "shainet_attn_attend_paged": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p,
+                                            C.c_longlong, C.c_void_p, C.c_longlong]),
+    "shainet_attn_step_paged": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p,
+                                          C.c_void_p]),
+    "shainet_attn_forward_paged": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, _i32p, _i32p, C.c_int, C.c_void_p, C.c_void_p,
+                                             C.c_void_p, C.c_void_p, C.c_int]),
     "shainet_attn_last_q_rot": (C.c_int, [C.c_void_p, _f32p, C.c_int]),
     "shainet_attn_describe_plan": (C.c_int, [C.c_int, C.c_int, C.c_int, C.c_int, _i32p, _i32p, _i32p]),
     "shainet_rope_apply": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_double, C.c_int]),
@@ -492,6 +511,208 @@ class AttnContext:
                 _check(rc)
 
         return call
+
+    def append_paged(self, cache, slots, positions, q, k, v, q_rot=None, layer=0):
+        """shainet_attn_append_paged: bias, QK-norm and rotation of rows of q, k and v (torch CUDA float32, rows may be
+        strided); K and V rows into slots[row] of a `PagedKVCache`, rotated queries into q_rot.  slots and positions are
+        int32 CUDA tensors, as `PagedKVCache.map_rows` writes them."""
+        import torch
+
+        rows = _ints(slots)
+        _ints(positions, rows)
+        _rows(q, rows, self.q_dim), _rows(k, rows, self.kv_dim), _rows(v, rows, self.kv_dim)
+        if q_rot is None:
+            q_rot = torch.empty((rows, self.q_dim), device=q.device)
+        if _rows(q_rot, rows, self.q_dim) != self.q_dim:
+            raise ArgumentError("q_rot must be contiguous")
+        _check(lib().shainet_attn_append_paged(self._h, cache._h, layer, _ptr(slots), _ptr(positions), rows, _ptr(q),
+                                               _stride(q), _ptr(k), _stride(k), _ptr(v), _stride(v), _ptr(q_rot)))
+        return q_rot
+
+    def attend_paged(self, cache, row_seqs, positions, q_rot, out=None, layer=0):
+        """shainet_attn_attend_paged: attention of rotated query rows over the first positions[row] + 1 rows of sequence
+        row_seqs[row] of a `PagedKVCache` (int32 CUDA tensors).  Rows whose row_seqs is no sequence are left alone in `out`."""
+        import torch
+
+        rows = _ints(row_seqs)
+        _ints(positions, rows)
+        _rows(q_rot, rows, self.q_dim)
+        if out is None:
+            out = torch.zeros((rows, self.q_dim), device=q_rot.device)
+            if out.is_cuda and torch.cuda.current_stream().cuda_stream != (self.stream or 0):
+                torch.cuda.current_stream().synchronize()  # (the zeros of rows left alone are there before the kernel writes)
+        _rows(out, rows, self.q_dim)
+        _check(lib().shainet_attn_attend_paged(self._h, cache._h, layer, _ptr(row_seqs), _ptr(positions), rows, _ptr(q_rot),
+                                               _stride(q_rot), _ptr(out), _stride(out)))
+        return out
+
+    def step_paged(self, cache, q, k, v, out, seq_ids=None, layer=0):
+        """shainet_attn_step_paged: one new row for each of q.shape[0] sequences of a `PagedKVCache` (seq_ids: int32 CUDA
+        tensor; None: the first ones), mapped, placed and attended by launches that can be recorded and replayed."""
+        n = q.shape[0]
+        if seq_ids is not None:
+            _ints(seq_ids, n)
+        for t, width in ((q, self.q_dim), (k, self.kv_dim), (v, self.kv_dim), (out, self.q_dim)):
+            if _rows(t, n, width) != width:
+                raise ArgumentError("q, k, v and out must be contiguous")
+        _check(lib().shainet_attn_step_paged(self._h, cache._h, layer, _ptr(seq_ids), n, _ptr(q), _ptr(k), _ptr(v), _ptr(out)))
+        return out
+
+    def forward_paged(self, cache, q, k, v, new_tokens, seq_ids=None, out=None, layer=0):
+        """`forward` over a `PagedKVCache`: any number of new rows for each of len(new_tokens) sequences.  numpy inputs run
+        the synchronous host-pointer mode and return numpy; torch CUDA tensors the asynchronous one."""
+        import numpy as np
+
+        n, rows = len(new_tokens), sum(new_tokens)
+        nt = (C.c_int * n)(*new_tokens)
+        ids = (C.c_int * n)(*seq_ids) if seq_ids is not None else None
+        if seq_ids is not None and len(seq_ids) != n:
+            raise ArgumentError("seq_ids and new_tokens differ in length")
+        if isinstance(q, np.ndarray):
+            q, k, v = (np.ascontiguousarray(a, np.float32) for a in (q, k, v))
+            if q.shape != (rows, self.q_dim) or k.shape != (rows, self.kv_dim) or v.shape != k.shape:
+                raise ArgumentError("q, k and v must be [%d, %d] and twice [%d, %d]" % (rows, self.q_dim, rows, self.kv_dim))
+            out, mem = np.empty((rows, self.q_dim), np.float32), MEM_HOST
+        else:
+            import torch
+
+            if out is None:
+                out = torch.empty_like(q)
+            for t, width in ((q, self.q_dim), (k, self.kv_dim), (v, self.kv_dim), (out, self.q_dim)):
+                if _rows(t, rows, width) != width:
+                    raise ArgumentError("q, k, v and out must be contiguous")
+            mem = MEM_DEVICE
+        _check(lib().shainet_attn_forward_paged(self._h, cache._h, layer, ids, nt, n, _ptr(q), _ptr(k), _ptr(v), _ptr(out), mem))
+        return out
+
+
+def _ints(t, n=None):
+    """Checks a CUDA int32 list (of n entries), as the calls on pages take them; returns its length."""
+    if not (hasattr(t, "is_cuda") and t.is_cuda and str(t.dtype) == "torch.int32" and t.is_contiguous() and n in (None, t.numel())):
+        raise ArgumentError("expected a contiguous int32 CUDA tensor" + ("" if n is None else " of %d entries" % n))
+    return t.numel()
+
+
+def _stride(t):
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _rows(t, n, width):
+    """Checks n CUDA float32 rows of `width` neighbouring numbers; returns the distance of two rows."""
+    if not (hasattr(t, "is_cuda") and t.is_cuda and str(t.dtype) == "torch.float32" and tuple(t.shape) == (n, width)
+            and (width == 1 or t.stride(1) == 1) and (n < 2 or t.stride(0) >= width)):
+        raise ArgumentError("expected a float32 CUDA tensor of %d rows of %d" % (n, width))
+    return _stride(t)
+
+
+class _PagedHandle:
+    """A shainet_paged_cache, destroyed when neither its PagedKVCache nor a tensor over its memory is left."""
+
+    def __init__(self, ctx, *geometry):
+        self.ctx, self.h = ctx, C.c_void_p()
+        _check(lib().shainet_paged_cache_create(C.byref(self.h), ctx._h, *geometry))
+
+    def __del__(self):
+        if self.h and getattr(self.ctx, "_h", None):
+            lib().shainet_paged_cache_destroy(self.h)
+        self.h = None
+
+
+class _DeviceArray:
+    """Device memory of a handle as torch.as_tensor takes it; the tensor keeps this and so the handle."""
+
+    def __init__(self, owner, address, shape, typestr):
+        self.owner = owner
+        self.__cuda_array_interface__ = {"data": (address, False), "shape": tuple(shape), "typestr": typestr, "version": 3}
+
+
+class PagedKVCache:
+    """KV cache in pages of page_rows rows that sequences take and give back as they grow and shrink; per layer K and V are
+    [n_pages][num_kv_heads][page_rows][head_dim] of dtype "f32", "bf16" or "f16".  The table of pages, the lengths and the
+    free pages lie on the device (`table`, `lens`, `free_pages`, `n_free`: tensors over the cache's own memory, which they
+    keep, as are `k` and `v` of layer 0 and `pages(layer)`)."""
+
+    DTYPES = {"f32": 0, "bf16": 1, "f16": 2}
+
+    def __init__(self, ctx, n_pages, page_rows, n_seqs, seq_pages, dtype="bf16", layers=1):
+        self._handle, self._views = None, {}
+        if dtype not in self.DTYPES:
+            raise ArgumentError("dtype must be one of %s" % ", ".join(self.DTYPES))
+        self.ctx = ctx
+        self._handle = _PagedHandle(ctx, layers, n_pages, page_rows, n_seqs, seq_pages, self.DTYPES[dtype])
+        self.n_pages, self.page_rows, self.n_seqs, self.seq_pages, self.dtype, self.layers = n_pages, page_rows, n_seqs, seq_pages, dtype, layers
+
+    def close(self):
+        """Lets go of the memory (which tensors over it keep)."""
+        self._handle, self._views = None, {}
+
+    @property
+    def _h(self):
+        return self._handle.h if self._handle else None
+
+    def _view(self, which, layer=0):
+        import torch
+
+        if not self._h:
+            raise ArgumentError("the cache is closed")
+        if (which, layer) not in self._views:
+            at = [C.c_void_p() for _ in range(6)]
+            _check(lib().shainet_paged_cache_arrays(self._h, layer, *(C.byref(a) for a in at)))
+            pool = (self.n_pages, self.ctx.num_kv_heads, self.page_rows, self.ctx.head_dim)
+            shape = (pool, pool, (self.n_seqs, self.seq_pages), (self.n_seqs,), (self.n_pages,), (1,))[which]
+            kind = ("<i4" if which > 1 else {"f32": "<f4", "bf16": "<i2", "f16": "<f2"}[self.dtype])
+            t = torch.as_tensor(_DeviceArray(self._handle, at[which].value, shape, kind), device="cuda")
+            self._views[which, layer] = t.view(torch.bfloat16) if which < 2 and self.dtype == "bf16" else t
+        return self._views[which, layer]
+
+    def pages(self, layer):
+        """(K, V) of one layer."""
+        return self._view(0, layer), self._view(1, layer)
+
+    k = property(lambda self: self._view(0))
+    v = property(lambda self: self._view(1))
+    table = property(lambda self: self._view(2))
+    lens = property(lambda self: self._view(3))
+    free_pages = property(lambda self: self._view(4))
+    n_free = property(lambda self: self._view(5))
+
+    def map_rows(self, delta, slots=None, positions=None, row_seqs=None, seq_ids=None):
+        """shainet_paged_cache_map_rows: sequences seq_ids (None: the first ones) change their lengths by delta rows; slots,
+        positions and row_seqs of the rows gained.  int32 CUDA tensors; the three lists may be left out where no row is gained."""
+        n, lists = _ints(delta), (slots, positions, row_seqs)
+        if seq_ids is not None:
+            _ints(seq_ids, n)
+        given = [t for t in lists if t is not None]
+        if len(given) not in (0, 3):
+            raise ArgumentError("slots, positions and row_seqs go together")
+        most = _ints(slots) if given else 0
+        for t in given:
+            _ints(t, most)
+        _check(lib().shainet_paged_cache_map_rows(self._h, _ptr(seq_ids), _ptr(delta), n, *((_ptr(t) for t in lists) if most else (None,) * 3), most))
+
+    def lengths_from_device(self):
+        """Waits, and takes the lengths over that calls on the device left."""
+        _check(lib().shainet_paged_cache_lengths_from_device(self._h))
+
+    def len(self, seq=0):
+        return lib().shainet_paged_cache_len(self._h, seq)
+
+    def free_page_count(self):
+        return lib().shainet_paged_cache_free_pages(self._h)
+
+    def truncate(self, seq, length):
+        _check(lib().shainet_paged_cache_truncate(self._h, seq, length))
+
+    def clear(self, seq=-1):
+        _check(lib().shainet_paged_cache_clear(self._h, seq))
+
+    def read(self, seq, kv_head, pos0, n, layer=0):
+        import numpy as np
+
+        k = np.empty((n, self.ctx.head_dim), np.float32)
+        v = np.empty((n, self.ctx.head_dim), np.float32)
+        _check(lib().shainet_paged_cache_read(self._h, layer, seq, kv_head, pos0, n, k.ctypes.data_as(_f32p), v.ctypes.data_as(_f32p)))
+        return k, v
 
 
 class KVCache:
