@@ -53,7 +53,7 @@ struct PagedAttendArgs {
   const int *row_seqs, *positions;
   int rows, H;
   float scale;
-  void *workspace;             // paged_attend_workspace() bytes, its first kPagedTickets words zero, which a launch leaves so
+  void *workspace;             // paged_attend_workspace() bytes, zero when allocated; a launch leaves its counts zero
 };
 size_t paged_attend_workspace(int hd);
 hipError_t launch_paged_attend(const PagedAttendArgs &a, const PagePool &p, hipStream_t stream);

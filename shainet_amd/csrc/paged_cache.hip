@@ -181,6 +181,8 @@ int append(shainet_attn_ctx *c, shainet_paged_cache *pc, int layer, const PrepAr
 
 int attend(shainet_attn_ctx *c, shainet_paged_cache *pc, int layer, const int *row_seqs, const int *positions, int rows,
            const float *q, long long q_stride, float *out, long long out_stride) {
+  if (rows * reach_of(pc) >= 1LL << 35)  // (tiles of 16 keys are counted in 32 bits)
+    return fail(SHAINET_HIP_ERR_ARGUMENT, "%d rows of up to %lld keys in one call: their product must stay below 2^35", rows, reach_of(pc));
   PagedAttendArgs a;
   a.q = q;
   a.out = out;
