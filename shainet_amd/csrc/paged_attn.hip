@@ -43,33 +43,47 @@ __device__ __forceinline__ float page_value(const void *pool, long long i) {
 }
 
 // Parts cross workgroups on XCDs whose L2 caches do not see each other's ordinary stores: relaxed atomic accesses at agent
-// scope write through and read past them.  A part is in memory before its count goes up (the wait for its stores).
+// scope write through.  A part is in memory before its count goes up (the wait for its stores).
 __device__ __forceinline__ void coherent_store(float *p, float v) {
   __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
+__device__ __forceinline__ void coherent_store4(float *p, f32x4 v) {  // the same, 16 bytes at a time
+  asm volatile("global_store_dwordx4 %0, %1, off sc1" : : "v"(p), "v"(v) : "memory");
+}
+
 __device__ __forceinline__ float coherent_load(const float *p) {
   return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
+__device__ __forceinline__ f32x4 coherent_load4(const float *p) {
+  typedef unsigned long long u64;
+  const u64 a = __hip_atomic_load((const u64 *)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  const u64 b = __hip_atomic_load((const u64 *)p + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  return f32x4{__builtin_bit_cast(float, (unsigned)a), __builtin_bit_cast(float, (unsigned)(a >> 32)),
+               __builtin_bit_cast(float, (unsigned)b), __builtin_bit_cast(float, (unsigned)(b >> 32))};
+}
 
-constexpr int kWaves = 4, kThreads = 64 * kWaves;
 constexpr int kCols = 16;  // query heads of a pair, at most: a larger group is several pairs
-constexpr int kMaxWorkgroups = 1024;
-// tiles of a span at least: a wavefront's first tile costs it a trip to memory, whose share this keeps down
-constexpr int kLeastSpan = 2 * kWaves;
+constexpr int kMaxWorkgroups = 512;
+constexpr int kTickets = 4 * kMaxWorkgroups;  // two places a workgroup, two levels
+constexpr int kTeam = 16;
+constexpr int kShortSpan = 32, kWavefrontTiles = 8, kOlderShare = 12;
 
 // What is laid out how for pages of a type and heads of up to HD.
 template <int DTYPE, int HD>
 struct Tile {
   static constexpr int E = DTYPE == kPageF32 ? 4 : 2;      // bytes of a number
-  static constexpr int S = DTYPE == kPageF32 ? 1 : 2;      // sixteens of keys
-  static constexpr int KEYS = 16 * S;
+  static constexpr int S = DTYPE == kPageF32 ? 1 : 2;      // sixteens of keys of a block
+  static constexpr int BLOCKS = HD == 64 ? 2 : 1;          // of a tile: 8 KiB of K at least
+  static constexpr int BLOCK_KEYS = 16 * S, KEYS = BLOCKS * BLOCK_KEYS;
   static constexpr int CHUNKS = HD * E / 64;               // 16-byte pieces of a K row per lane
   static constexpr int PER = 16 / E;                       // numbers in one
   static constexpr int VEC = HD / 16 < PER ? HD / 16 : PER;  // neighbouring columns of a V row per lane
   static constexpr int PIECES = HD / (16 * VEC);           // ... how often
   static constexpr int WORDS = VEC * E / 4;                // of 4 bytes, in one
   static constexpr int PARTS = DTYPE == kPageF32 ? 1 : DTYPE == kPageBf16 ? 3 : 2;  // of a float operand
-  static constexpr int PER_CU = HD == 64 ? 3 : HD == 128 ? 2 : 1;  // workgroups of a compute unit
+  static constexpr int WAVES = 4;                          // of a workgroup
+  static constexpr int PER_CU = HD == 256 ? 1 : 2;         // workgroups of a compute unit
+  static constexpr int WHOLE = 12;                                 // tiles of a pair that is not worth being cut
 };
 
 template <int WORDS>
@@ -83,116 +97,151 @@ struct Words<4> {
   typedef u32x4 T;
 };
 
-// Where the spans lie.
-struct Plan {
-  int total, span;
-};
-
-struct Segment {
-  int row, seq, len, first, last;  // tiles [first, last) of the row's
-  int head, cols;                  // query heads head .. head + cols - 1
-  int kv;
-  int begins, ends;                // of the pair's tiles in the stream
-};
-
 template <int DTYPE, int HD, bool PAD>
 struct Wave {
   using T = Tile<DTYPE, HD>;
   typedef typename Words<T::WORDS>::T VWords;
   static constexpr int KEYS_EACH = 4 * T::S;  // of a quarter
 
+  // A tile in registers, or on its way there.
+  struct Held {
+    u32x4 k[T::BLOCKS][T::S][T::CHUNKS];
+    VWords v[T::BLOCKS][KEYS_EACH][T::PIECES];
+    bool in[T::BLOCKS];  // whether this lane's V rows, which are the keys of its scores, lie in the pool
+  };
+  // This wavefront's share of a row of queries: chunks `first`, first + step, ...
+  static constexpr int SHARE = (T::CHUNKS + T::WAVES - 1) / T::WAVES;
+  struct Raw {
+    f32x4 x[SHARE][T::PER / 4];
+  };
+
   const PagePool &p;
+  const u32x4 *q;  // the queries' parts in LDS, [PARTS][CHUNKS][64]
   const int lane, m, j;
   const int hd;
-  u32x4 k[T::S][T::CHUNKS];
-  VWords v[KEYS_EACH][T::PIECES];
-  u32x4 q[T::PARTS][DTYPE == kPageF32 ? T::CHUNKS : T::CHUNKS];
+  Held held;
   f32x4 acc[T::PIECES][T::VEC];
   float top, sum;  // running maximum of the scores in log2 units, and this lane's share of the sum
   float c;         // scores to log2 units
   int down;        // float16: the queries were multiplied by 2^down
-  // pages of this lane's K row and V rows in the tile to be asked for next, and whether those V rows, which are the keys of this lane's
-  // scores, lie in the pool; of the tile in registers, too
-  int k_page, v_page;
-  bool v_in, v_in_next;
+  struct Pages {
+    int k[T::BLOCKS], v[T::BLOCKS];  // of this lane's K row and V rows in a tile
+  };
+  Pages now, next;  // of a walk's first tile, and of the tile to be asked for next
   const int *table;
   int last_page, len;
   const char *k_base, *v_base;
 
-  __device__ __forceinline__ Wave(const PagePool &pool) : p(pool), lane(threadIdx.x & 63), m(lane & 15), j(lane >> 4), hd(PAD ? pool.hd : HD) {}
+  __device__ __forceinline__ Wave(const PagePool &pool, float scale)
+      : p(pool), lane(threadIdx.x & 63), m(lane & 15), j(lane >> 4), hd(PAD ? pool.hd : HD), c(scale * 1.44269504088896340736f), down(0) {}
 
-  __device__ __forceinline__ void look_up(int tile) {
-    const int k0 = tile * T::KEYS;
-    const int kp = table[min((k0 + (m >> 2) * KEYS_EACH) >> p.shift, last_page)];
-    const int vp = table[min((k0 + j * KEYS_EACH) >> p.shift, last_page)];
-    k_page = (unsigned)kp < (unsigned)p.n_pages ? kp : 0;
-    v_in_next = (unsigned)vp < (unsigned)p.n_pages;
-    v_page = v_in_next ? vp : 0;
-  }
-
-  __device__ __forceinline__ const char *row_at(const char *base, int page, int key) const {
-    const long long row = ((long long)page * p.KV << p.shift) + (key & ((1 << p.shift) - 1));
-    return base + row * (hd * T::E);
-  }
-  __device__ __forceinline__ void ask_k(int tile) {
+  // (behind the last tile: its last page again)
+  __device__ __forceinline__ void look_up(Pages &at_page, int tile) const {
 #pragma unroll
-    for (int s = 0; s < T::S; ++s) {
-      const char *row = row_at(k_base, k_page, tile * T::KEYS + (m >> 2) * KEYS_EACH + 4 * s + (m & 3));
-#pragma unroll
-      for (int u = 0; u < T::CHUNKS; ++u) {
-        int at = (u * 4 + j) * 16;
-        if (PAD) at = at < hd * T::E ? at : 0;
-        k[s][u] = __builtin_nontemporal_load((const u32x4 *)(row + at));
-      }
+    for (int b = 0; b < T::BLOCKS; ++b) {
+      const int k0 = tile * T::KEYS + b * T::BLOCK_KEYS;
+      at_page.k[b] = table[min((k0 + (m >> 2) * KEYS_EACH) >> p.shift, last_page)];
+      at_page.v[b] = table[min((k0 + j * KEYS_EACH) >> p.shift, last_page)];
     }
   }
-  __device__ __forceinline__ void ask_v(int tile) {
-    const char *row = row_at(v_base, v_page, tile * T::KEYS + j * KEYS_EACH);
+  __device__ __forceinline__ const char *row_at(const char *base, int page, int key) const {
+    const long long row = ((long long)((unsigned)page < (unsigned)p.n_pages ? page : 0) * p.KV << p.shift) + (key & ((1 << p.shift) - 1));
+    return base + row * (hd * T::E);
+  }
+  // (anew each time, so that there is no register for each load's offset over the loop)
+  __device__ __forceinline__ int row_bytes() const {
+    int n = hd * T::E;
+    if (PAD) asm volatile("" : "+s"(n));
+    return n;
+  }
+  __device__ __forceinline__ void ask_k(const Pages &at_page, int tile) {
+    const int bytes = row_bytes();
 #pragma unroll
-    for (int r = 0; r < KEYS_EACH; ++r)
+    for (int b = 0; b < T::BLOCKS; ++b)
 #pragma unroll
-      for (int u = 0; u < T::PIECES; ++u) {
-        int at = (T::VEC * m + 16 * T::VEC * u) * T::E;
-        if (PAD) at = at < hd * T::E ? at : 0;
-        v[r][u] = __builtin_nontemporal_load((const VWords *)(row + r * (hd * T::E) + at));
+      for (int s = 0; s < T::S; ++s) {
+        const char *row = row_at(k_base, at_page.k[b], tile * T::KEYS + b * T::BLOCK_KEYS + (m >> 2) * KEYS_EACH + 4 * s + (m & 3));
+#pragma unroll
+        for (int u = 0; u < T::CHUNKS; ++u) {
+          int at = (u * 4 + j) * 16;
+          if (PAD) at = at < bytes ? at : 0;
+          held.k[b][s][u] = __builtin_nontemporal_load((const u32x4 *)(row + at));
+        }
       }
-    v_in = v_in_next;
+  }
+  __device__ __forceinline__ void ask_v(const Pages &at_page, int tile) {
+    const int bytes = row_bytes();
+#pragma unroll
+    for (int b = 0; b < T::BLOCKS; ++b) {
+      const char *row = row_at(v_base, at_page.v[b], tile * T::KEYS + b * T::BLOCK_KEYS + j * KEYS_EACH);
+      held.in[b] = (unsigned)at_page.v[b] < (unsigned)p.n_pages;
+#pragma unroll
+      for (int r = 0; r < KEYS_EACH; ++r)
+#pragma unroll
+        for (int u = 0; u < T::PIECES; ++u) {
+          int at = (T::VEC * m + 16 * T::VEC * u) * T::E;
+          if (PAD) at = at < bytes ? at : 0;
+          held.v[b][r][u] = __builtin_nontemporal_load((const VWords *)(row + r * (hd * T::E) + at));
+        }
+    }
   }
 
   // The queries as B operands: chunk u of quarter j is d = (4 u + j) PER .. + PER - 1, as K's.
-  __device__ __forceinline__ void load_queries(const float *rows, int cols, float scale) {
-    f32x4 x[T::CHUNKS][T::PER / 4];
+  __device__ __forceinline__ f32x4 query(const float *rows, int cols, int u, int w) const {
+    const int d = (4 * u + j) * T::PER + 4 * w;
+    f32x4 x = {0, 0, 0, 0};
+    if (m < cols && (!PAD || d < hd) && u < T::CHUNKS)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = rows[m * hd + d + e];
+    return x;
+  }
+  __device__ __forceinline__ void ask_queries(Raw &raw, const float *rows, int cols, int first, int step) const {
+#pragma unroll
+    for (int i = 0; i < SHARE; ++i)
+#pragma unroll
+      for (int w = 0; w < T::PER / 4; ++w) raw.x[i][w] = query(rows, cols, first + i * step, w);
+  }
+  // float16 parts hold 22 bits of a number between two of them, down to 2^-24: the largest of a row is brought to 2^14 .. 2^15
+  __device__ __forceinline__ void find_down(const float *rows, int cols) {
     float most = 0.0f;
 #pragma unroll
     for (int u = 0; u < T::CHUNKS; ++u)
 #pragma unroll
       for (int w = 0; w < T::PER / 4; ++w) {
-        const int d = (4 * u + j) * T::PER + 4 * w;
-        x[u][w] = f32x4{0, 0, 0, 0};
-        if (m < cols && (!PAD || d < hd))
-#pragma unroll
-          for (int e = 0; e < 4; ++e) x[u][w][e] = rows[m * hd + d + e];
-        most = fmaxf(fmaxf(most, fmaxf(fabsf(x[u][w].x), fabsf(x[u][w].y))), fmaxf(fabsf(x[u][w].z), fabsf(x[u][w].w)));
+        const f32x4 x = query(rows, cols, u, w);
+        most = fmaxf(most, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))));
       }
-    c = scale * 1.44269504088896340736f;
-    down = 0;
-    if constexpr (DTYPE == kPageF16) {
-      // two float16 parts hold 22 bits of a number, down to 2^-24: the largest of the row is brought to 2^14 .. 2^15
-      most = max_across_quarters(most);
-      down = most > 0.0f && most < INFINITY ? 15 - __builtin_amdgcn_frexp_expf(most) : 0;
+    most = max_across_quarters(most);
+    down = most > 0.0f && most < INFINITY ? 15 - __builtin_amdgcn_frexp_expf(most) : 0;
+  }
+  __device__ __forceinline__ void put_query(u32x4 *to, const f32x4 (&x)[T::PER / 4], int u) const {
+    u32x4 part[T::PARTS];
+    if constexpr (DTYPE == kPageF32) {
+      part[0] = __builtin_bit_cast(u32x4, x[0]);
+    } else if constexpr (DTYPE == kPageBf16) {
+      split_octet(x[0], x[1], part[0], part[1], part[2]);
+    } else {
+      float y[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = ldexpf(x[e >> 2][e & 3], down);
+      split_f16(y, part[0], part[1]);
     }
 #pragma unroll
-    for (int u = 0; u < T::CHUNKS; ++u) {
-      if constexpr (DTYPE == kPageF32) {
-        q[0][u] = __builtin_bit_cast(u32x4, x[u][0]);
-      } else if constexpr (DTYPE == kPageBf16) {
-        split_octet(x[u][0], x[u][1], q[0][u], q[1][u], q[2][u]);
-      } else {
-        float y[8];
+    for (int i = 0; i < T::PARTS; ++i) to[(i * T::CHUNKS + u) * 64 + lane] = part[i];
+  }
+  __device__ __forceinline__ void put_queries(u32x4 *to, const Raw &raw, int first, int step) const {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = ldexpf(x[u][e >> 2][e & 3], down);
-        split_f16(y, q[0][u], q[1][u]);
-      }
+    for (int i = 0; i < SHARE; ++i)
+      if (first + i * step < T::CHUNKS) put_query(to, raw.x[i], first + i * step);
+  }
+  // ... all of them by this wavefront, for itself
+  __device__ __forceinline__ void own_queries(u32x4 *to, const float *rows, int cols) const {
+#pragma unroll
+    for (int u = 0; u < T::CHUNKS; ++u) {
+      f32x4 x[T::PER / 4];
+#pragma unroll
+      for (int w = 0; w < T::PER / 4; ++w) x[w] = query(rows, cols, u, w);
+      put_query(to, x, u);
     }
   }
   __device__ __forceinline__ static void split_f16(const float (&y)[8], u32x4 &high, u32x4 &low) {
@@ -210,83 +259,103 @@ struct Wave {
       return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), x, 0, 0, 0);
   }
 
-  __device__ __forceinline__ void begin(const Segment &s) {
-    len = s.len;
-    table = p.table + (long long)s.seq * p.seq_pages;
+  // Looks up the first two of a sequence's tiles first, first + step, ...; `ask` asks for the first, if it is below last.
+  __device__ __forceinline__ void start(int seq, int keys, int kv, int first, int step) {
+    len = keys;
+    table = p.table + (long long)seq * p.seq_pages;
     last_page = (len - 1) >> p.shift;
-    const long long head = ((long long)s.kv << p.shift) * (hd * T::E);
+    const long long head = ((long long)kv << p.shift) * (hd * T::E);
     k_base = (const char *)p.k + head;
     v_base = (const char *)p.v + head;
-    top = -INFINITY;
-    sum = 0.0f;
+    look_up(now, first);
+    look_up(next, first + step);
+  }
+  __device__ __forceinline__ void ask(int first, int last) {
+    // (the entries are waited for here, where nothing is behind them yet)
 #pragma unroll
-    for (int u = 0; u < T::PIECES; ++u)
-#pragma unroll
-      for (int e = 0; e < T::VEC; ++e) acc[u][e] = f32x4{0, 0, 0, 0};
+    for (int b = 0; b < T::BLOCKS; ++b) asm volatile("" : "+v"(now.k[b]), "+v"(now.v[b]), "+v"(next.k[b]), "+v"(next.v[b]));
+    if (first >= last) return;
+    ask_k(now, first);
+    ask_v(now, first);
   }
 
-  // Tiles first, first + step, ... below last.
-  __device__ __forceinline__ void walk(int first, int last, int step) {
-    if (first >= last) return;
-    look_up(first);
-    ask_k(first);
-    ask_v(first);
-    if (first + step < last) look_up(first + step);
-    for (int tile = first; tile < last; tile += step) {
-      const int next = tile + step;
-      f32x4 x[T::S];
+  // What is held becomes part of sums and outputs.  MORE: and its place is asked to hold tile `then`, whose pages were looked
+  // up, those of `after` before it.  (Loads come back in order and are waited for by their number: how many are on their way has to be the same
+  // however the code is reached, and an address that came by a load behind others would wait for all of them.)
+  template <bool MORE>
+  __device__ __forceinline__ void take(int tile, int then, int after) {
+    f32x4 x[T::BLOCKS][T::S];
 #pragma unroll
-      for (int s = 0; s < T::S; ++s) {
-        x[s] = f32x4{0, 0, 0, 0};
+    for (int b = 0; b < T::BLOCKS; ++b)
 #pragma unroll
-        for (int part = T::PARTS - 1; part >= 0; --part)
+      for (int s = 0; s < T::S; ++s) x[b][s] = f32x4{0, 0, 0, 0};
 #pragma unroll
-          for (int u = 0; u < T::CHUNKS; ++u) {
+    for (int part = T::PARTS - 1; part >= 0; --part)
+#pragma unroll
+      for (int u = 0; u < T::CHUNKS; ++u) {
+        const u32x4 mine = q[(part * T::CHUNKS + u) * 64 + lane];
+#pragma unroll
+        for (int b = 0; b < T::BLOCKS; ++b)
+#pragma unroll
+          for (int s = 0; s < T::S; ++s) {
             if constexpr (DTYPE == kPageF32) {
-              const f32x4 a = __builtin_bit_cast(f32x4, k[s][u]), b = __builtin_bit_cast(f32x4, q[0][u]);
+              const f32x4 k = __builtin_bit_cast(f32x4, held.k[b][s][u]), y = __builtin_bit_cast(f32x4, mine);
 #pragma unroll
-              for (int e = 0; e < 4; ++e) x[s] = mfma_f32_16(a[e], b[e], x[s]);
+              for (int e = 0; e < 4; ++e) x[b][s] = mfma_f32_16(k[e], y[e], x[b][s]);
             } else {
-              x[s] = mfma16(k[s][u], q[part][u], x[s]);
+              x[b][s] = mfma16(held.k[b][s][u], mine, x[b][s]);
             }
           }
       }
-      if (next < last) ask_k(next);
-      if constexpr (DTYPE == kPageF16)
+    const Pages its = next;
+    if constexpr (MORE) {
+      look_up(next, after);
+      ask_k(its, then);
+    }
+    // keys behind the sequence's end or in no page: no score, and a value that is no number would not vanish at weight 0
+    bool whole = true;
 #pragma unroll
-        for (int s = 0; s < T::S; ++s)
+    for (int b = 0; b < T::BLOCKS; ++b) whole = whole && held.in[b];
+    float most = -INFINITY;
+    if (__any(!whole || (tile + 1) * T::KEYS > len)) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) x[s][i] = ldexpf(x[s][i], -down);
-      // keys behind the sequence's end or in no page: no score, and a value that is no number would not vanish at weight 0
-      const int key = tile * T::KEYS + j * KEYS_EACH;
-      if (__any(!v_in || key + KEYS_EACH > len)) {
+      for (int b = 0; b < T::BLOCKS; ++b) {
+        const int key = tile * T::KEYS + b * T::BLOCK_KEYS + j * KEYS_EACH;
 #pragma unroll
         for (int r = 0; r < KEYS_EACH; ++r)
-          if (!v_in || key + r >= len) {
-            x[r >> 2][r & 3] = -INFINITY;
+          if (!held.in[b] || key + r >= len) {
+            x[b][r >> 2][r & 3] = -INFINITY;
 #pragma unroll
-            for (int u = 0; u < T::PIECES; ++u) v[r][u] = VWords{};
+            for (int u = 0; u < T::PIECES; ++u) held.v[b][r][u] = VWords{};
           }
       }
-      float most = fmaxf(fmaxf(x[0].x, x[0].y), fmaxf(x[0].z, x[0].w));
-      if constexpr (T::S == 2) most = fmaxf(most, fmaxf(fmaxf(x[1].x, x[1].y), fmaxf(x[1].z, x[1].w)));
-      most = max_across_quarters(most) * c;
-      if (__any(most > top)) {
-        const float now = fmaxf(top, most);
-        const float fade = now == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top - now);
-        top = now;
-        sum *= fade;
+    }
 #pragma unroll
-        for (int u = 0; u < T::PIECES; ++u)
+    for (int b = 0; b < T::BLOCKS; ++b)
 #pragma unroll
-          for (int e = 0; e < T::VEC; ++e) acc[u][e] *= fade;
+      for (int r = 0; r < KEYS_EACH; ++r) {
+        if constexpr (DTYPE == kPageF16) x[b][r >> 2][r & 3] = ldexpf(x[b][r >> 2][r & 3], -down);
+        most = fmaxf(most, x[b][r >> 2][r & 3]);
       }
-      // (float16 parts of a weight: lifted by 2^15, as the queries are; the sum is lifted with them)
-      const float from = top == -INFINITY ? 0.0f : DTYPE == kPageF16 ? top - 15.0f : top;
+    most = max_across_quarters(most) * c;
+    if (__any(most > top)) {
+      const float now = fmaxf(top, most);
+      const float fade = now == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top - now);
+      top = now;
+      sum *= fade;
+#pragma unroll
+      for (int u = 0; u < T::PIECES; ++u)
+#pragma unroll
+        for (int e = 0; e < T::VEC; ++e) acc[u][e] *= fade;
+    }
+    // (float16 parts of a weight: lifted by 2^15, as the queries are; the sum is lifted with them)
+    const float from = top == -INFINITY ? 0.0f : DTYPE == kPageF16 ? top - 15.0f : top;
+#pragma unroll
+    for (int b = 0; b < T::BLOCKS; ++b) {
       float w[KEYS_EACH];
 #pragma unroll
       for (int r = 0; r < KEYS_EACH; ++r) {
-        w[r] = __builtin_amdgcn_exp2f(fmaf(x[r >> 2][r & 3], c, -from));
+        w[r] = __builtin_amdgcn_exp2f(fmaf(x[b][r >> 2][r & 3], c, -from));
         sum += w[r];
       }
       if constexpr (DTYPE == kPageF32) {
@@ -294,7 +363,7 @@ struct Wave {
         for (int r = 0; r < KEYS_EACH; ++r)
 #pragma unroll
           for (int u = 0; u < T::PIECES; ++u) {
-            const f32x4 columns = __builtin_bit_cast(f32x4, v[r][u]);
+            const f32x4 columns = __builtin_bit_cast(f32x4, held.v[b][r][u]);
 #pragma unroll
             for (int e = 0; e < T::VEC; ++e) acc[u][e] = mfma_f32_16(columns[e], w[r], acc[u][e]);
           }
@@ -311,180 +380,451 @@ struct Wave {
             u32x4 column;
 #pragma unroll
             for (int r = 0; r < 4; ++r)
-              column[r] = __builtin_amdgcn_perm(v[2 * r + 1][u][e >> 1], v[2 * r][u][e >> 1], e & 1 ? 0x07060302u : 0x05040100u);
+              column[r] = __builtin_amdgcn_perm(held.v[b][2 * r + 1][u][e >> 1], held.v[b][2 * r][u][e >> 1], e & 1 ? 0x07060302u : 0x05040100u);
 #pragma unroll
             for (int part = T::PARTS - 1; part >= 0; --part) acc[u][e] = mfma16(column, weights[part], acc[u][e]);
           }
       }
-      if (next < last) {
-        ask_v(next);
-        if (next + step < last) look_up(next + step);
-      }
     }
+    if constexpr (MORE) ask_v(its, then);
+  }
+
+  // Sums and outputs of those tiles.
+  __device__ __forceinline__ void walk(int first, int last, int step) {
+    top = -INFINITY;
+    sum = 0.0f;
+#pragma unroll
+    for (int u = 0; u < T::PIECES; ++u)
+#pragma unroll
+      for (int e = 0; e < T::VEC; ++e) acc[u][e] = f32x4{0, 0, 0, 0};
+    if (first >= last) return;
+    int tile = first;
+#pragma unroll 1
+    for (; tile + step < last; tile += step) take<true>(tile, tile + step, tile + 2 * step);
+    take<false>(tile, 0, 0);
   }
 };
 
+// Sum, or maximum (of numbers that are not negative), over the lanes up to this one.
+template <typename F>
+__device__ __forceinline__ int scan_lanes(int x, F two) {
+  x = two(x, __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false));  // row_shr 1, 2, 4, 8
+  x = two(x, __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false));
+  x = two(x, __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false));
+  x = two(x, __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false));
+  x = two(x, __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false));  // row_bcast 15, 31
+  return two(x, __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false));
+}
+__device__ __forceinline__ int sum_lanes(int x) {
+  return scan_lanes(x, [](int a, int b) { return a + b; });
+}
+__device__ __forceinline__ int max_lanes(int x) {
+  return scan_lanes(x, [](int a, int b) { return max(a, b); });
+}
+
+// How a launch shares out its work; the same for all workgroups, each of which makes it for itself.
+enum { kSpans, kChunks, kWavefronts };
+
 template <int DTYPE, int HD, bool PAD>
-__global__ __launch_bounds__(kThreads, (Tile<DTYPE, HD>::PER_CU)) void paged_attend_kernel(PagedAttendArgs a, PagePool p) {
+__global__ __launch_bounds__((64 * Tile<DTYPE, HD>::WAVES), (Tile<DTYPE, HD>::WAVES / 4 * Tile<DTYPE, HD>::PER_CU)) void paged_attend_kernel(PagedAttendArgs a, PagePool p) {
   using T = Tile<DTYPE, HD>;
-  constexpr int STRIDE = HD + 4;
-  __shared__ int starts[kMaxPagedSeqs + 1];                 // tiles of one kv head in the rows before
-  __shared__ float outs[kWaves][kCols][STRIDE];
-  __shared__ float tops[kWaves][kCols], sums[kWaves][kCols];
-  __shared__ int scan[kWaves], last_one;
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  constexpr int WAVES = T::WAVES, THREADS = 64 * WAVES, STRIDE = HD + 4;
+  constexpr int NEAR = 512;                                 // rows whose lengths stay at hand
+  __shared__ int starts[kMaxPagedSeqs + 1];                 // units of one kv head in the rows before: tiles or chunks
+  __shared__ int seqs[NEAR], lens[NEAR];
+  // the queries, and the wavefronts' outputs behind them; of wavefronts that go their own ways, the queries of each
+  constexpr int QUERIES = T::PARTS * T::CHUNKS * 64 * 4, OUTS = WAVES * kCols * STRIDE;
+  __shared__ __align__(16) float shared[QUERIES + (OUTS > (WAVES - 1) * QUERIES ? OUTS : (WAVES - 1) * QUERIES)];
+  auto outs = [&](int v, int n, int d) { return shared + QUERIES + (v * kCols + n) * STRIDE + d; };
+  __shared__ float tops[WAVES][kCols], sums[WAVES][kCols];
+  __shared__ int scan[WAVES], held[WAVES], longest[WAVES], last_one;
+  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  // (values from LDS that are the same in all lanes are said to be: they live in scalar registers then)
+  auto same = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
   const int hd = PAD ? p.hd : HD;
   const int g = a.H / p.KV, per_kv = (g + kCols - 1) / kCols, pairs = p.KV * per_kv;
   const int most_keys = (int)min((long long)p.seq_pages << p.shift, 0x3fffffffLL);
+  const int wgs = (int)gridDim.x;
 
-  // sums of the rows' tiles; outputs of rows without keys
-  {
-    const int each = (a.rows + kThreads - 1) / kThreads;
-    int mine = 0;
-    for (int i = 0; i < each; ++i) {
-      const int r = t * each + i;
-      int tiles = 0;
-      if (r < a.rows && (unsigned)a.row_seqs[r] < (unsigned)p.n_seqs)
-        tiles = (max(0, min(a.positions[r], most_keys - 1) + 1) + T::KEYS - 1) / T::KEYS;
-      if (r < a.rows) starts[r] = mine;
-      mine += tiles;
+  // rows of a length that has a sequence; -1: a row to be left alone
+  auto length_of = [&](int r, int &seq) {
+    seq = a.row_seqs[r];
+    return (unsigned)seq < (unsigned)p.n_seqs ? max(0, min(a.positions[r], most_keys - 1) + 1) : -1;
+  };
+  auto known_length = [&](int r) {
+    int seq;
+    return r < NEAR ? lens[r] : length_of(r, seq);
+  };
+  auto tiles_of = [](int len) { return (max(len, 0) + T::KEYS - 1) / T::KEYS; };
+  // the rows' tiles in all, how many rows have any, and the most of one.  Up to a wavefront's lanes of rows: every wavefront
+  // makes them for itself (they all write the same to LDS, and each reads what it wrote), and nobody waits at a barrier.
+  const bool few = a.rows <= 64;
+  const int each = few ? 1 : (a.rows + THREADS - 1) / THREADS, first_row = few ? lane : t * each;
+  int row_tiles = 0, some = 0, most = 0;
+  for (int i = 0; i < each; ++i) {
+    const int r = first_row + i;
+    if (r >= a.rows) break;
+    int seq;
+    const int len = length_of(r, seq), tiles = tiles_of(len);
+    if (r < NEAR) {
+      seqs[r] = seq;
+      lens[r] = len;
     }
-    int inclusive = mine;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int x = __shfl_up(inclusive, d);
-      if (lane >= d) inclusive += x;
-    }
-    if (lane == 63) scan[wave] = inclusive;
-    __syncthreads();
-    int before = inclusive - mine, all = 0;
-    for (int w = 0; w < kWaves; ++w) {
-      before += w < wave ? scan[w] : 0;
-      all += scan[w];
-    }
-    for (int i = 0; i < each; ++i) {
-      const int r = t * each + i;
-      if (r < a.rows) starts[r] += before;
-    }
-    if (t == 0) starts[a.rows] = all;
-    __syncthreads();
+    row_tiles += tiles;
+    some += tiles > 0 ? 1 : 0;
+    most = max(most, tiles);
   }
-  for (int r = blockIdx.x; r < a.rows; r += gridDim.x)
-    if (starts[r + 1] == starts[r] && (unsigned)a.row_seqs[r] < (unsigned)p.n_seqs)
-      for (int i = t; i < a.H * hd; i += kThreads) a.out[r * a.out_stride + i] = 0.0f;
+  row_tiles = __builtin_amdgcn_readlane(sum_lanes(row_tiles), 63);
+  some = few ? (int)__builtin_popcountll(__ballot(some)) : __builtin_amdgcn_readlane(sum_lanes(some), 63);
+  most = __builtin_amdgcn_readlane(max_lanes(most), 63);
+  if (!few) {
+    if (lane == 0) {
+      scan[wave] = row_tiles;
+      held[wave] = some;
+      longest[wave] = most;
+    }
+    __syncthreads();
+    row_tiles = some = most = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+      row_tiles += scan[w];
+      some += held[w];
+      most = max(most, longest[w]);
+    }
+  }
+  row_tiles = same(row_tiles);
+  some = same(some);
+  most = same(most);
+  // outputs of rows without keys
+  for (int r = blockIdx.x; r < a.rows; r += wgs)
+    if (known_length(r) == 0)
+      for (int i = t; i < a.H * hd; i += THREADS) a.out[r * a.out_stride + i] = 0.0f;
+  const long long total = (long long)row_tiles * pairs, n_pairs = (long long)some * pairs;
+  int mode = kSpans;
+  long long unit = max(1LL, (total + wgs - 1) / wgs);  // tiles of a span, or of a chunk at most
+  if (n_pairs > wgs && most <= kWavefrontTiles) {
+    mode = kWavefronts;
+  } else if (unit < kShortSpan && n_pairs <= wgs) {
+    // chunks of pairs, one a workgroup: sum of ceil(tiles / unit) <= total / unit + pairs
+    mode = kChunks;
+    unit = n_pairs < wgs && most > T::WHOLE ? max((total + (wgs - n_pairs) - 1) / (wgs - n_pairs), (long long)WAVES) : most;
+  }
+  if (mode != kWavefronts) {  // units of one kv head before each row
+    auto units_of = [&](int r) {
+      const int tiles = tiles_of(known_length(r));
+      return mode == kSpans ? tiles : (tiles + (int)unit - 1) / (int)unit;
+    };
+    if (few) {
+      const int mine = lane < a.rows ? units_of(lane) : 0, upto = sum_lanes(mine);
+      if (lane < a.rows) starts[lane + 1] = upto;
+      if (lane == 0) starts[0] = 0;
+    } else {
+      int mine = 0;
+      for (int i = 0; i < each && first_row + i < a.rows; ++i) mine += units_of(first_row + i);
+      const int upto = sum_lanes(mine);
+      __syncthreads();  // (`scan` has been read)
+      if (lane == 63) scan[wave] = upto;
+      __syncthreads();
+      int before = upto - mine;
+      for (int w = 0; w < wave; ++w) before += scan[w];
+      for (int i = 0; i < each && first_row + i < a.rows; ++i) {
+        starts[first_row + i] = before;
+        before += units_of(first_row + i);
+        if (first_row + i == a.rows - 1) starts[a.rows] = before;
+      }
+      __syncthreads();
+    }
+  }
 
-  const long long total = (long long)starts[a.rows] * pairs;
-  const long long span = max((long long)kLeastSpan, (total + gridDim.x - 1) / gridDim.x);
-  long long at = blockIdx.x * span;
-  const long long end = min(total, at + span);
-  if (at >= end) return;
-  int row;
-  {
+  const long long all_units = mode == kWavefronts ? (long long)a.rows * pairs : (long long)same(starts[a.rows]) * pairs;
+  // The first half of the workgroups are the first on their compute units, whose requests go before the others': with equal
+  // spans they ended at 88 us and the others at 105 to 118 (16 sequences of 2048 to 8192 keys, float32).
+  const int half = wgs / 2;
+  const long long longer = unit, shorter = unit;
+  auto span_begin = [&](int wg) { return min(wg, half) * longer + max(wg - half, 0) * shorter; };
+  auto span_of = [&](long long tile) {
+    return (int)(tile < half * longer ? tile / longer : half + (tile - half * longer) / shorter);
+  };
+  long long at = mode == kSpans ? span_begin(blockIdx.x) : mode == kChunks ? blockIdx.x : blockIdx.x + (long long)wgs * wave;
+  const long long end = mode == kSpans ? min(all_units, span_begin(blockIdx.x + 1)) : mode == kChunks ? min(all_units, at + 1) : all_units;
+  unsigned *tickets = (unsigned *)a.workspace;
+  float *parts = (float *)(tickets + kTickets);
+  constexpr int PART = kCols * HD + 4 * kCols;  // a workgroup has two: of the pair that it begins with, and of the one that goes on behind it
+  int row = 0;
+  if (mode != kWavefronts && at < end) {
     int lo = 0, hi = a.rows - 1;
-    while (lo < hi) {  // the last row that begins at or before it and has tiles
+    while (lo < hi) {  // the last row that begins at or before it
       const int mid = (lo + hi + 1) >> 1;
-      if ((long long)starts[mid] * pairs <= at)
+      if ((long long)same(starts[mid]) * pairs <= at)
         lo = mid;
       else
         hi = mid - 1;
     }
     row = lo;
   }
-  unsigned *tickets = (unsigned *)a.workspace;
-  float *parts = (float *)(tickets + kMaxWorkgroups);
-  constexpr int PART = kCols * (HD + 2);  // a workgroup has two: of the pair that it begins with, and of the one that goes on behind it
-  Wave<DTYPE, HD, PAD> w(p);
-  while (at < end) {
-    while (starts[row + 1] == starts[row] || (long long)starts[row + 1] * pairs <= at) ++row;
-    row = __builtin_amdgcn_readfirstlane(row);
-    Segment s;
-    const int tiles = __builtin_amdgcn_readfirstlane(starts[row + 1] - starts[row]);
-    const long long of_row = (long long)__builtin_amdgcn_readfirstlane(starts[row]) * pairs;
-    const int pair = (int)((at - of_row) / tiles);
-    const long long begins = of_row + (long long)pair * tiles, ends = begins + tiles;
-    s.row = row;
-    s.seq = a.row_seqs[row];
-    s.len = min(a.positions[row], most_keys - 1) + 1;
-    s.first = (int)(at - begins);
-    s.last = (int)(min(end, ends) - begins);
-    s.kv = pair / per_kv;
-    s.head = s.kv * g + (pair - s.kv * per_kv) * kCols;
-    s.cols = min(kCols, g - (pair - s.kv * per_kv) * kCols);
-    w.begin(s);
-    w.load_queries(a.q + s.row * a.q_stride + (long long)s.head * hd, s.cols, a.scale);
-    w.walk(s.first + wave, s.last, kWaves);
+  // A pair, and which of its tiles are this workgroup's (wavefront's); first_wg .. last_wg: whose the pair is
+  struct Segment {
+    int row, seq, len, pair, first, last;
+    int first_wg, last_wg;
+    bool late, first_late;  // the pair begins in this workgroup's span (in first_wg's) but not with it: its part is the second there
+  };
+  auto next_segment = [&](Segment &s) {
+    while (at < end) {
+      if (mode == kWavefronts) {
+        row = (int)(at / pairs);
+        s.pair = (int)(at - (long long)row * pairs);
+        at += (long long)wgs * WAVES;
+      } else {
+        while ((long long)same(starts[row + 1]) * pairs <= at) ++row;
+      }
+      row = same(row);
+      s.row = row;
+      if (row < NEAR) {
+        s.seq = same(seqs[row]);
+        s.len = same(lens[row]);
+      } else {
+        s.len = length_of(row, s.seq);
+      }
+      const int tiles = tiles_of(s.len);
+      s.first = 0;
+      s.last = tiles;
+      if (mode == kWavefronts) {
+        if (tiles == 0) continue;
+        s.pair = same(s.pair);
+        return true;
+      }
+      const int units = same(starts[row + 1] - starts[row]);
+      const long long of_row = (long long)same(starts[row]) * pairs;
+      s.pair = same((int)((at - of_row) / units));
+      const long long begins = of_row + (long long)s.pair * units;
+      const int from = (int)(at - begins);
+      if (mode == kSpans) {
+        s.first = from;
+        s.last = (int)(min(end, begins + units) - begins);
+        at += s.last - s.first;
+        s.first_wg = span_of(begins);
+        s.last_wg = span_of(begins + units - 1);
+        s.late = begins > span_begin(blockIdx.x);
+        s.first_late = begins > span_begin(s.first_wg);
+      } else {  // equal shares
+        s.first = (int)((long long)tiles * from / units);
+        s.last = (int)((long long)tiles * (from + 1) / units);
+        at += 1;
+        s.first_wg = (int)begins;
+        s.last_wg = (int)begins + units - 1;
+        s.late = s.first_late = false;
+      }
+      return true;
+    }
+    return false;
+  };
+
+  Wave<DTYPE, HD, PAD> w(p, a.scale);
+  const bool alone = mode == kWavefronts;
+  const int step = alone ? 1 : WAVES, mine = alone ? 0 : wave;
+  u32x4 *const queries = (u32x4 *)shared + (alone ? wave * (QUERIES / 4) : 0);
+  w.q = queries;
+  auto head_of = [&](const Segment &s) { return s.pair / per_kv * g + s.pair % per_kv * kCols; };
+  auto cols_of = [&](const Segment &s) { return min(kCols, g - s.pair % per_kv * kCols); };
+  auto rows_of = [&](const Segment &s) { return a.q + s.row * a.q_stride + (long long)head_of(s) * hd; };
+  typename Wave<DTYPE, HD, PAD>::Raw raw;
+  // a segment's table entries and queries are asked for first, then its first tile
+  auto start = [&](const Segment &s) {
+    w.start(s.seq, s.len, s.pair / per_kv, s.first + mine, step);
+    if (!alone) w.ask_queries(raw, rows_of(s), cols_of(s), wave, WAVES);
+    w.ask(s.first + mine, s.last);
+  };
+  auto put_queries = [&](const Segment &s) {
+    if constexpr (DTYPE == kPageF16) w.find_down(rows_of(s), cols_of(s));
+    if (alone)
+      w.own_queries(queries, rows_of(s), cols_of(s));
+    else
+      w.put_queries(queries, raw, wave, WAVES);
+  };
+  Segment s;
+  bool more = next_segment(s);
+  if (more) {
+    start(s);
+    put_queries(s);
+  }
+  __syncthreads();
+  while (more) {
+    const int cols = cols_of(s);
+    float *out = a.out + s.row * a.out_stride + (long long)head_of(s) * hd;
+    w.walk(s.first + mine, s.last, step);
+    // the next segment's first tile is on its way while this one's outputs are put together
+    const Segment now = s;
+    more = next_segment(s);
+    if (more) start(s);
+    const float its_sum = sum_across_quarters(w.sum);
+    if (alone) {
+      const float over = its_sum == 0.0f ? 0.0f : 1.0f / its_sum;
+      if (w.m < cols)
+#pragma unroll
+        for (int u = 0; u < T::PIECES; ++u)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int e = 0; e < T::VEC; ++e) {
+              const int d = T::VEC * (4 * w.j + i) + 16 * T::VEC * u + e;
+              if (!PAD || d < hd) out[w.m * hd + d] = w.acc[u][e][i] * over;
+            }
+      if (more) put_queries(s);
+      continue;
+    }
 
     // the wavefronts' parts, on one maximum
-    const float mine = sum_across_quarters(w.sum);
     if (lane < kCols) {
       tops[wave][lane] = w.top;
-      sums[wave][lane] = mine;
+      sums[wave][lane] = its_sum;
     }
     __syncthreads();
     float top = -INFINITY;
-    for (int i = 0; i < kWaves; ++i) top = fmaxf(top, tops[i][w.m]);
+#pragma unroll
+    for (int i = 0; i < WAVES; ++i) top = fmaxf(top, tops[i][w.m]);
     const float fade = w.top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(w.top - top);
+    if (w.m < cols)
 #pragma unroll
-    for (int u = 0; u < T::PIECES; ++u)
+      for (int u = 0; u < T::PIECES; ++u)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int e = 0; e < T::VEC; ++e)
-          outs[wave][w.m][T::VEC * (4 * w.j + i) + 16 * T::VEC * u + e] = w.acc[u][e][i] * fade;
+          for (int e = 0; e < T::VEC; e += 4)
+            *(f32x4 *)outs(wave, w.m, T::VEC * (4 * w.j + i) + 16 * T::VEC * u + e) =
+                f32x4{w.acc[u][e][i], w.acc[u][e + 1][i], w.acc[u][e + 2][i], w.acc[u][e + 3][i]} * fade;
     __syncthreads();
-    const bool whole = begins == at && ends <= end;
-    const long long first_wg = begins / span, last_wg = (ends - 1) / span;
-    // (a pair that begins in a workgroup's span but not with it, and does not end there, is the span's last: its second part)
-    auto part_of = [&](long long wg) { return parts + (wg * 2 + (wg == first_wg && begins != wg * span ? 1 : 0)) * PART; };
-    float *part = part_of(blockIdx.x);
-    for (int i = t; i < s.cols * hd; i += kThreads) {
-      const int n = i / hd, d = i - n * hd;
-      float x = 0.0f, l = 0.0f, best = -INFINITY;
+    if (more) put_queries(s);  // (nobody reads the old ones any more)
+    const bool whole = now.first_wg == now.last_wg;
+    const int fours = cols * hd / 4;
+    // Parts of a pair: k = 0 .. n_parts - 1, each in its workgroup's first or second place.
+    const int n_parts = now.last_wg - now.first_wg + 1;
+    auto place_of = [&](int k) { return (now.first_wg + k) * 2 + (k == 0 && now.first_late ? 1 : 0); };
+    float *part = parts + (blockIdx.x * 2 + (now.late ? 1 : 0)) * PART;
+    for (int i = t; i < fours; i += THREADS) {
+      const int n = 4 * i / hd, d = 4 * i - n * hd;
+      f32x4 x = {0, 0, 0, 0};
 #pragma unroll
-      for (int v = 0; v < kWaves; ++v) {
-        x += outs[v][n][d];
-        best = fmaxf(best, tops[v][n]);
-      }
+      for (int v = 0; v < WAVES; ++v) x += *(const f32x4 *)outs(v, n, d);
+      if (whole || d == 0) {
+        float best = -INFINITY, l = 0.0f;
 #pragma unroll
-      for (int v = 0; v < kWaves; ++v) l += sums[v][n] * (tops[v][n] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(tops[v][n] - best));
-      if (whole) {
-        a.out[s.row * a.out_stride + (long long)(s.head + n) * hd + d] = l == 0.0f ? 0.0f : x / l;
-      } else {
-        coherent_store(part + n * (HD + 2) + d, x);
-        if (d == 0) {
-          coherent_store(part + n * (HD + 2) + HD, best);
-          coherent_store(part + n * (HD + 2) + HD + 1, l);
+        for (int v = 0; v < WAVES; ++v) best = fmaxf(best, tops[v][n]);
+#pragma unroll
+        for (int v = 0; v < WAVES; ++v) l += sums[v][n] * (tops[v][n] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(tops[v][n] - best));
+        if (whole) {
+          const float over = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) out[4 * i + e] = x[e] * over;
+        } else {
+          coherent_store(part + kCols * HD + n, best);
+          coherent_store(part + kCols * HD + kCols + n, l);
         }
       }
+      if (!whole) coherent_store4(part + 4 * i, x);
     }
-    if (!whole) {
+    // Up to kTeam parts are added up by the last one's workgroup; of more, each so many first, by the last of theirs, into the
+    // place of their first, and then what that leaves.
+    int first_part = 0, gap = 1, count = n_parts;
+    if (n_parts > kTeam) {
+      first_part = (blockIdx.x - now.first_wg) / kTeam * kTeam;
+      count = min(kTeam, n_parts - first_part);
+    }
+#pragma unroll 1
+    for (bool going = !whole; going;) {
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       __syncthreads();
       if (t == 0) {
-        const unsigned others = (unsigned)(last_wg - first_wg);
-        const unsigned before = __hip_atomic_fetch_add(tickets + first_wg, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        last_one = before == others;
-        if (before == others) __hip_atomic_store(tickets + first_wg, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        unsigned *ticket = tickets + (gap == 1 ? 0 : 2 * kMaxWorkgroups) + place_of(first_part);
+        const unsigned before = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        last_one = before == (unsigned)count - 1;
+        if (last_one) __hip_atomic_store(ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       }
       __syncthreads();
-      if (last_one) {
-        for (int i = t; i < s.cols * hd; i += kThreads) {
-          const int n = i / hd, d = i - n * hd;
-          float best = -INFINITY;
-          for (long long wg = first_wg; wg <= last_wg; ++wg) best = fmaxf(best, coherent_load(part_of(wg) + n * (HD + 2) + HD));
-          float x = 0.0f, l = 0.0f;
-          for (long long wg = first_wg; wg <= last_wg; ++wg) {
-            const float *from = part_of(wg) + n * (HD + 2);
-            const float its = coherent_load(from + HD), fades = its == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(its - best);
-            x = fmaf(coherent_load(from + d), fades, x);
-            l = fmaf(coherent_load(from + HD + 1), fades, l);
+      if (!last_one) break;
+      const bool final = gap > 1 || n_parts <= kTeam;
+      // A thread adds up four neighbouring outputs over the parts, with a running maximum as a wavefront does over tiles; where
+      // there are fewer outputs than threads, teams of threads take every so-manieth part each.
+      const int teams = max(1, THREADS / fours), team = teams > 1 ? t / fours : 0;
+      float *work = shared + QUERIES;  // [teams][fours][6]
+      float *to = parts + place_of(first_part) * PART;
+      auto finish = [&](int i, f32x4 x, float best, float l) {
+        if (final) {
+          const float over = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) out[4 * i + e] = x[e] * over;
+        } else {
+          const int n = 4 * i / hd;
+          coherent_store4(to + 4 * i, x);
+          if (4 * i == n * hd) {
+            coherent_store(to + kCols * HD + 2 * kCols + n, best);  // (others still read its own)
+            coherent_store(to + kCols * HD + 3 * kCols + n, l);
           }
-          a.out[s.row * a.out_stride + (long long)(s.head + n) * hd + d] = l == 0.0f ? 0.0f : x / l;
+        }
+      };
+      const int peaks = kCols * HD + (gap > 1 ? 2 * kCols : 0);  // maxima and sums of parts, or of what they were added up to
+#pragma unroll 1
+      for (int i = teams > 1 ? t - team * fours : t; i < fours && team < teams; i += teams > 1 ? fours : THREADS) {
+        const int n = 4 * i / hd;
+        float best = -INFINITY, l = 0.0f;
+        f32x4 x = {0, 0, 0, 0};
+        constexpr int SOME = 8;
+#pragma unroll 1
+        for (int k = team; k < count; k += SOME * teams) {
+          float its[SOME], its_l[SOME];
+          f32x4 its_x[SOME];
+#pragma unroll
+          for (int z = 0; z < SOME; ++z) {
+            const float *from = parts + place_of(first_part + min(k + z * teams, count - 1) * gap) * PART;
+            its[z] = coherent_load(from + peaks + n);
+            its_l[z] = coherent_load(from + peaks + kCols + n);
+            its_x[z] = coherent_load4(from + 4 * i);
+          }
+          float higher = best;
+#pragma unroll
+          for (int z = 0; z < SOME; ++z) higher = fmaxf(higher, its[z]);
+          const float less = best == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(best - higher);
+          best = higher;
+          l *= less;
+          x *= less;
+#pragma unroll
+          for (int z = 0; z < SOME; ++z) {  // (no branch: loads behind one would wait for the one before)
+            const float f = its[z] == -INFINITY || k + z * teams >= count ? 0.0f : __builtin_amdgcn_exp2f(its[z] - higher);
+            l = fmaf(its_l[z], f, l);
+            x += its_x[z] * f;
+          }
+        }
+        if (teams == 1) {
+          finish(i, x, best, l);
+        } else {
+          float *mine_at = work + (team * fours + i) * 6;
+          mine_at[0] = best;
+          mine_at[1] = l;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) mine_at[2 + e] = x[e];
         }
       }
+      if (teams > 1) {
+        __syncthreads();
+        for (int i = t; i < fours; i += THREADS) {
+          float best = -INFINITY, l = 0.0f;
+          for (int k = 0; k < teams; ++k) best = fmaxf(best, work[(k * fours + i) * 6]);
+          f32x4 x = {0, 0, 0, 0};
+          for (int k = 0; k < teams; ++k) {
+            const float *from = work + (k * fours + i) * 6;
+            const float f = from[0] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(from[0] - best);
+            l = fmaf(from[1], f, l);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = fmaf(from[2 + e], f, x[e]);
+          }
+          finish(i, x, best, l);
+        }
+      }
+      going = !final;
+      first_part = 0;
+      gap = kTeam;
+      count = (n_parts + kTeam - 1) / kTeam;
     }
     __syncthreads();  // the next segment writes to LDS
-    at += s.last - s.first;
   }
 }
 
@@ -514,7 +854,7 @@ __global__ __launch_bounds__(256) void page_gather_kernel(PagePool p, int seq, i
 
 size_t paged_attend_workspace(int hd) {
   const int tile = hd <= 64 ? 64 : hd <= 128 ? 128 : 256;
-  return kMaxWorkgroups * sizeof(unsigned) + (size_t)kMaxWorkgroups * 2 * kCols * (tile + 2) * sizeof(float);
+  return kTickets * sizeof(unsigned) + (size_t)kMaxWorkgroups * 2 * kCols * (tile + 4) * sizeof(float);
 }
 
 namespace {
@@ -523,7 +863,7 @@ hipError_t launch_attend(const PagedAttendArgs &a, const PagePool &p, hipStream_
   constexpr int wgs = 256 * Tile<DTYPE, HD>::PER_CU;
   static_assert(wgs <= kMaxWorkgroups, "counts and parts");
   const auto kernel = p.hd == HD ? paged_attend_kernel<DTYPE, HD, false> : paged_attend_kernel<DTYPE, HD, true>;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)wgs), dim3(kThreads), 0, stream, a, p);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)wgs), dim3(64 * Tile<DTYPE, HD>::WAVES), 0, stream, a, p);
   return hipGetLastError();
 }
 template <int DTYPE>

@@ -44,6 +44,7 @@ def build_library(force=True):
 
 
 _lib = None
+_F32 = _I32 = None  # torch's types, once the library is loaded
 
 _SIGNATURES = {
     "shainet_hip_last_error": (C.c_char_p, []),
@@ -196,8 +197,11 @@ def lib():
         # A process may hold only one HIP runtime.  PyTorch ships its own copy under the
         # same soname; when torch is installed it must be loaded first so that this
         # library binds to that copy instead of bringing in a second one.
+        global _F32, _I32
         try:
-            import torch  # noqa: F401
+            import torch
+
+            _F32, _I32 = torch.float32, torch.int32
         except ImportError:
             pass
         L = C.CDLL(_SO)
@@ -512,50 +516,56 @@ class AttnContext:
 
         return call
 
+    # The calls of a decode step are made hundreds of times a second and each takes a few microseconds on the device: their
+    # checks look at every argument once and nothing else is done (append_paged: 10.3 us a call, 6 of them checks, before).
+
     def append_paged(self, cache, slots, positions, q, k, v, q_rot=None, layer=0):
         """shainet_attn_append_paged: bias, QK-norm and rotation of rows of q, k and v (torch CUDA float32, rows may be
         strided); K and V rows into slots[row] of a `PagedKVCache`, rotated queries into q_rot.  slots and positions are
         int32 CUDA tensors, as `PagedKVCache.map_rows` writes them."""
-        import torch
-
         rows = _ints(slots)
         _ints(positions, rows)
-        _rows(q, rows, self.q_dim), _rows(k, rows, self.kv_dim), _rows(v, rows, self.kv_dim)
+        qs, ks, vs = _rows(q, rows, self.q_dim), _rows(k, rows, self.kv_dim), _rows(v, rows, self.kv_dim)
         if q_rot is None:
-            q_rot = torch.empty((rows, self.q_dim), device=q.device)
-        if _rows(q_rot, rows, self.q_dim) != self.q_dim:
+            q_rot = q.new_empty((rows, self.q_dim))
+        elif _rows(q_rot, rows, self.q_dim) != self.q_dim:
             raise ArgumentError("q_rot must be contiguous")
-        _check(lib().shainet_attn_append_paged(self._h, cache._h, layer, _ptr(slots), _ptr(positions), rows, _ptr(q),
-                                               _stride(q), _ptr(k), _stride(k), _ptr(v), _stride(v), _ptr(q_rot)))
+        rc = _lib.shainet_attn_append_paged(self._h, cache._h, layer, slots.data_ptr(), positions.data_ptr(), rows, q.data_ptr(), qs,
+                                            k.data_ptr(), ks, v.data_ptr(), vs, q_rot.data_ptr())
+        if rc:
+            _check(rc)
         return q_rot
 
     def attend_paged(self, cache, row_seqs, positions, q_rot, out=None, layer=0):
         """shainet_attn_attend_paged: attention of rotated query rows over the first positions[row] + 1 rows of sequence
         row_seqs[row] of a `PagedKVCache` (int32 CUDA tensors).  Rows whose row_seqs is no sequence are left alone in `out`."""
-        import torch
-
         rows = _ints(row_seqs)
         _ints(positions, rows)
-        _rows(q_rot, rows, self.q_dim)
+        stride = _rows(q_rot, rows, self.q_dim)
         if out is None:
-            out = torch.zeros((rows, self.q_dim), device=q_rot.device)
-            if out.is_cuda and torch.cuda.current_stream().cuda_stream != (self.stream or 0):
+            import torch
+
+            out = q_rot.new_zeros((rows, self.q_dim))
+            if torch.cuda.current_stream().cuda_stream != (self.stream or 0):
                 torch.cuda.current_stream().synchronize()  # (the zeros of rows left alone are there before the kernel writes)
-        _rows(out, rows, self.q_dim)
-        _check(lib().shainet_attn_attend_paged(self._h, cache._h, layer, _ptr(row_seqs), _ptr(positions), rows, _ptr(q_rot),
-                                               _stride(q_rot), _ptr(out), _stride(out)))
+        rc = _lib.shainet_attn_attend_paged(self._h, cache._h, layer, row_seqs.data_ptr(), positions.data_ptr(), rows, q_rot.data_ptr(),
+                                            stride, out.data_ptr(), _rows(out, rows, self.q_dim))
+        if rc:
+            _check(rc)
         return out
 
     def step_paged(self, cache, q, k, v, out, seq_ids=None, layer=0):
         """shainet_attn_step_paged: one new row for each of q.shape[0] sequences of a `PagedKVCache` (seq_ids: int32 CUDA
         tensor; None: the first ones), mapped, placed and attended by launches that can be recorded and replayed."""
-        n = q.shape[0]
+        n, qd, kd = q.shape[0], self.q_dim, self.kv_dim
         if seq_ids is not None:
             _ints(seq_ids, n)
-        for t, width in ((q, self.q_dim), (k, self.kv_dim), (v, self.kv_dim), (out, self.q_dim)):
-            if _rows(t, n, width) != width:
-                raise ArgumentError("q, k, v and out must be contiguous")
-        _check(lib().shainet_attn_step_paged(self._h, cache._h, layer, _ptr(seq_ids), n, _ptr(q), _ptr(k), _ptr(v), _ptr(out)))
+        if (_rows(q, n, qd), _rows(k, n, kd), _rows(v, n, kd), _rows(out, n, qd)) != (qd, kd, kd, qd):
+            raise ArgumentError("q, k, v and out must be contiguous")
+        rc = _lib.shainet_attn_step_paged(self._h, cache._h, layer, None if seq_ids is None else seq_ids.data_ptr(), n, q.data_ptr(),
+                                          k.data_ptr(), v.data_ptr(), out.data_ptr())
+        if rc:
+            _check(rc)
         return out
 
     def forward_paged(self, cache, q, k, v, new_tokens, seq_ids=None, out=None, layer=0):
@@ -588,21 +598,28 @@ class AttnContext:
 
 def _ints(t, n=None):
     """Checks a CUDA int32 list (of n entries), as the calls on pages take them; returns its length."""
-    if not (hasattr(t, "is_cuda") and t.is_cuda and str(t.dtype) == "torch.int32" and t.is_contiguous() and n in (None, t.numel())):
-        raise ArgumentError("expected a contiguous int32 CUDA tensor" + ("" if n is None else " of %d entries" % n))
-    return t.numel()
-
-
-def _stride(t):
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    try:
+        size = t.numel()
+        if t.dtype is _I32 and t.is_cuda and t.is_contiguous() and (n is None or n == size):
+            return size
+    except (AttributeError, TypeError):
+        pass
+    raise ArgumentError("expected a contiguous int32 CUDA tensor" + ("" if n is None else " of %d entries" % n))
 
 
 def _rows(t, n, width):
     """Checks n CUDA float32 rows of `width` neighbouring numbers; returns the distance of two rows."""
-    if not (hasattr(t, "is_cuda") and t.is_cuda and str(t.dtype) == "torch.float32" and tuple(t.shape) == (n, width)
-            and (width == 1 or t.stride(1) == 1) and (n < 2 or t.stride(0) >= width)):
-        raise ArgumentError("expected a float32 CUDA tensor of %d rows of %d" % (n, width))
-    return _stride(t)
+    try:
+        if t.dtype is _F32 and t.is_cuda and t.shape == (n, width):
+            far, near = t.stride()
+            if near == 1 or width == 1:
+                if n < 2:
+                    return width
+                if far >= width:
+                    return far
+    except (AttributeError, TypeError):
+        pass
+    raise ArgumentError("expected a float32 CUDA tensor of %d rows of %d" % (n, width))
 
 
 class _PagedHandle:
@@ -613,7 +630,7 @@ class _PagedHandle:
         _check(lib().shainet_paged_cache_create(C.byref(self.h), ctx._h, *geometry))
 
     def __del__(self):
-        if self.h and getattr(self.ctx, "_h", None):
+        if self.h and getattr(self.ctx, "_h", None) and lib is not None:  # (None: the interpreter is on its way out)
             lib().shainet_paged_cache_destroy(self.h)
         self.h = None
 
@@ -635,20 +652,17 @@ class PagedKVCache:
     DTYPES = {"f32": 0, "bf16": 1, "f16": 2}
 
     def __init__(self, ctx, n_pages, page_rows, n_seqs, seq_pages, dtype="bf16", layers=1):
-        self._handle, self._views = None, {}
+        self._h, self._handle, self._views = None, None, {}
         if dtype not in self.DTYPES:
             raise ArgumentError("dtype must be one of %s" % ", ".join(self.DTYPES))
         self.ctx = ctx
         self._handle = _PagedHandle(ctx, layers, n_pages, page_rows, n_seqs, seq_pages, self.DTYPES[dtype])
+        self._h = self._handle.h
         self.n_pages, self.page_rows, self.n_seqs, self.seq_pages, self.dtype, self.layers = n_pages, page_rows, n_seqs, seq_pages, dtype, layers
 
     def close(self):
         """Lets go of the memory (which tensors over it keep)."""
-        self._handle, self._views = None, {}
-
-    @property
-    def _h(self):
-        return self._handle.h if self._handle else None
+        self._h, self._handle, self._views = None, None, {}
 
     def _view(self, which, layer=0):
         import torch
@@ -679,16 +693,22 @@ class PagedKVCache:
     def map_rows(self, delta, slots=None, positions=None, row_seqs=None, seq_ids=None):
         """shainet_paged_cache_map_rows: sequences seq_ids (None: the first ones) change their lengths by delta rows; slots,
         positions and row_seqs of the rows gained.  int32 CUDA tensors; the three lists may be left out where no row is gained."""
-        n, lists = _ints(delta), (slots, positions, row_seqs)
+        n = _ints(delta)
         if seq_ids is not None:
             _ints(seq_ids, n)
-        given = [t for t in lists if t is not None]
-        if len(given) not in (0, 3):
-            raise ArgumentError("slots, positions and row_seqs go together")
-        most = _ints(slots) if given else 0
-        for t in given:
-            _ints(t, most)
-        _check(lib().shainet_paged_cache_map_rows(self._h, _ptr(seq_ids), _ptr(delta), n, *((_ptr(t) for t in lists) if most else (None,) * 3), most))
+            seq_ids = seq_ids.data_ptr()
+        if slots is None or positions is None or row_seqs is None:
+            if not (slots is positions is row_seqs):
+                raise ArgumentError("slots, positions and row_seqs go together")
+            rc = _lib.shainet_paged_cache_map_rows(self._h, seq_ids, delta.data_ptr(), n, None, None, None, 0)
+        else:
+            most = _ints(slots)
+            _ints(positions, most)
+            _ints(row_seqs, most)
+            rc = _lib.shainet_paged_cache_map_rows(self._h, seq_ids, delta.data_ptr(), n, slots.data_ptr(), positions.data_ptr(),
+                                                   row_seqs.data_ptr(), most)
+        if rc:
+            _check(rc)
 
     def lengths_from_device(self):
         """Waits, and takes the lengths over that calls on the device left."""

@@ -62,7 +62,7 @@ def test_lists_that_are_no_device_lists_are_refused(lib):
     import torch
 
     cache = hip.PagedKVCache.__new__(hip.PagedKVCache)
-    cache._handle, cache._views, cache.ctx = None, {}, None
+    cache._h, cache._handle, cache._views, cache.ctx = None, None, {}, None
     for bad in (torch.zeros(3, dtype=torch.int32), np.zeros(3, np.int32), torch.zeros(3)):
         with pytest.raises(hip.ArgumentError):
             cache.map_rows(bad)
