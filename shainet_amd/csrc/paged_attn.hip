@@ -66,18 +66,18 @@ constexpr int kCols = 16;  // query heads of a pair, at most: a larger group is 
 constexpr int kMaxWorkgroups = 512;
 constexpr int kTickets = 4 * kMaxWorkgroups;  // two places a workgroup, two levels
 constexpr int kTeam = 16;
-constexpr int kShortSpan = 32, kWavefrontTiles = 8, kOlderShare = 12;
+constexpr int kShortSpan = 32, kWavefrontTiles = 8;
 
 // What is laid out how for pages of a type and heads of up to HD.
 template <int DTYPE, int HD>
 struct Tile {
   static constexpr int E = DTYPE == kPageF32 ? 4 : 2;      // bytes of a number
   static constexpr int S = DTYPE == kPageF32 ? 1 : 2;      // sixteens of keys of a block
-  static constexpr int BLOCKS = HD == 64 ? 2 : 1;          // of a tile: 8 KiB of K at least
+  static constexpr int BLOCKS = 1;                         // of a tile
   static constexpr int BLOCK_KEYS = 16 * S, KEYS = BLOCKS * BLOCK_KEYS;
   static constexpr int CHUNKS = HD * E / 64;               // 16-byte pieces of a K row per lane
   static constexpr int PER = 16 / E;                       // numbers in one
-  static constexpr int VEC = HD / 16 < PER ? HD / 16 : PER;  // neighbouring columns of a V row per lane
+  static constexpr int VEC = HD == 96 ? 3 * PER / 4 : HD / 16 < PER ? HD / 16 : PER;  // neighbouring columns of a V row per lane
   static constexpr int PIECES = HD / (16 * VEC);           // ... how often
   static constexpr int WORDS = VEC * E / 4;                // of 4 bytes, in one
   static constexpr int PARTS = DTYPE == kPageF32 ? 1 : DTYPE == kPageBf16 ? 3 : 2;  // of a float operand
@@ -91,6 +91,10 @@ struct Words;
 template <>
 struct Words<2> {
   typedef u32x2 T;
+};
+template <>
+struct Words<3> {
+  typedef unsigned T __attribute__((ext_vector_type(3), aligned(4)));  // (pieces of 12 bytes)
 };
 template <>
 struct Words<4> {
@@ -151,7 +155,7 @@ struct Wave {
   // (anew each time, so that there is no register for each load's offset over the loop)
   __device__ __forceinline__ int row_bytes() const {
     int n = hd * T::E;
-    if (PAD) asm volatile("" : "+s"(n));
+    if (PAD) asm volatile("" : "+v"(n));
     return n;
   }
   __device__ __forceinline__ void ask_k(const Pages &at_page, int tile) {
@@ -363,7 +367,8 @@ struct Wave {
         for (int r = 0; r < KEYS_EACH; ++r)
 #pragma unroll
           for (int u = 0; u < T::PIECES; ++u) {
-            const f32x4 columns = __builtin_bit_cast(f32x4, held.v[b][r][u]);
+            typedef float Columns __attribute__((ext_vector_type(T::WORDS)));
+            const Columns columns = __builtin_bit_cast(Columns, held.v[b][r][u]);
 #pragma unroll
             for (int e = 0; e < T::VEC; ++e) acc[u][e] = mfma_f32_16(columns[e], w[r], acc[u][e]);
           }
@@ -537,16 +542,8 @@ __global__ __launch_bounds__((64 * Tile<DTYPE, HD>::WAVES), (Tile<DTYPE, HD>::WA
   }
 
   const long long all_units = mode == kWavefronts ? (long long)a.rows * pairs : (long long)same(starts[a.rows]) * pairs;
-  // The first half of the workgroups are the first on their compute units, whose requests go before the others': with equal
-  // spans they ended at 88 us and the others at 105 to 118 (16 sequences of 2048 to 8192 keys, float32).
-  const int half = wgs / 2;
-  const long long longer = unit, shorter = unit;
-  auto span_begin = [&](int wg) { return min(wg, half) * longer + max(wg - half, 0) * shorter; };
-  auto span_of = [&](long long tile) {
-    return (int)(tile < half * longer ? tile / longer : half + (tile - half * longer) / shorter);
-  };
-  long long at = mode == kSpans ? span_begin(blockIdx.x) : mode == kChunks ? blockIdx.x : blockIdx.x + (long long)wgs * wave;
-  const long long end = mode == kSpans ? min(all_units, span_begin(blockIdx.x + 1)) : mode == kChunks ? min(all_units, at + 1) : all_units;
+  long long at = mode == kSpans ? blockIdx.x * unit : mode == kChunks ? blockIdx.x : blockIdx.x + (long long)wgs * wave;
+  const long long end = mode == kSpans ? min(all_units, at + unit) : mode == kChunks ? min(all_units, at + 1) : all_units;
   unsigned *tickets = (unsigned *)a.workspace;
   float *parts = (float *)(tickets + kTickets);
   constexpr int PART = kCols * HD + 4 * kCols;  // a workgroup has two: of the pair that it begins with, and of the one that goes on behind it
@@ -602,10 +599,10 @@ __global__ __launch_bounds__((64 * Tile<DTYPE, HD>::WAVES), (Tile<DTYPE, HD>::WA
         s.first = from;
         s.last = (int)(min(end, begins + units) - begins);
         at += s.last - s.first;
-        s.first_wg = span_of(begins);
-        s.last_wg = span_of(begins + units - 1);
-        s.late = begins > span_begin(blockIdx.x);
-        s.first_late = begins > span_begin(s.first_wg);
+        s.first_wg = (int)(begins / unit);
+        s.last_wg = (int)((begins + units - 1) / unit);
+        s.late = begins > blockIdx.x * unit;
+        s.first_late = begins > s.first_wg * unit;
       } else {  // equal shares
         s.first = (int)((long long)tiles * from / units);
         s.last = (int)((long long)tiles * (from + 1) / units);
@@ -619,6 +616,11 @@ __global__ __launch_bounds__((64 * Tile<DTYPE, HD>::WAVES), (Tile<DTYPE, HD>::WA
     return false;
   };
 
+  // Of two workgroups on a compute unit the first one's requests go before the other's: with equal spans the first ones ended at
+  // 77 to 100 us and the others at 108 to 118 (16 sequences of 2048 to 8192 keys, float32).  The others' instructions go
+  // first, therefore: half to one per cent of most launches.  (Spans of unequal lengths, or short ones for whoever is
+  // ready, cost more in parts of pairs than they gave: 110 -> 113 and 121 us.)
+  if (T::PER_CU == 2 && (int)blockIdx.x >= wgs / 2) __builtin_amdgcn_s_setprio(3);
   Wave<DTYPE, HD, PAD> w(p, a.scale);
   const bool alone = mode == kWavefronts;
   const int step = alone ? 1 : WAVES, mine = alone ? 0 : wave;
@@ -689,9 +691,8 @@ __global__ __launch_bounds__((64 * Tile<DTYPE, HD>::WAVES), (Tile<DTYPE, HD>::WA
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
-          for (int e = 0; e < T::VEC; e += 4)
-            *(f32x4 *)outs(wave, w.m, T::VEC * (4 * w.j + i) + 16 * T::VEC * u + e) =
-                f32x4{w.acc[u][e][i], w.acc[u][e + 1][i], w.acc[u][e + 2][i], w.acc[u][e + 3][i]} * fade;
+          for (int e = 0; e < T::VEC; ++e)
+            *outs(wave, w.m, T::VEC * (4 * w.j + i) + 16 * T::VEC * u + e) = w.acc[u][e][i] * fade;
     __syncthreads();
     if (more) put_queries(s);  // (nobody reads the old ones any more)
     const bool whole = now.first_wg == now.last_wg;
@@ -853,7 +854,7 @@ __global__ __launch_bounds__(256) void page_gather_kernel(PagePool p, int seq, i
 }  // namespace
 
 size_t paged_attend_workspace(int hd) {
-  const int tile = hd <= 64 ? 64 : hd <= 128 ? 128 : 256;
+  const int tile = hd <= 64 ? 64 : hd <= 96 ? 96 : hd <= 128 ? 128 : 256;
   return kTickets * sizeof(unsigned) + (size_t)kMaxWorkgroups * 2 * kCols * (tile + 4) * sizeof(float);
 }
 
@@ -868,7 +869,7 @@ hipError_t launch_attend(const PagedAttendArgs &a, const PagePool &p, hipStream_
 }
 template <int DTYPE>
 hipError_t launch_attend(const PagedAttendArgs &a, const PagePool &p, hipStream_t stream) {
-  return p.hd <= 64 ? launch_attend<DTYPE, 64>(a, p, stream) : p.hd <= 128 ? launch_attend<DTYPE, 128>(a, p, stream) : launch_attend<DTYPE, 256>(a, p, stream);
+  return p.hd <= 64 ? launch_attend<DTYPE, 64>(a, p, stream) : p.hd <= 96 ? launch_attend<DTYPE, 96>(a, p, stream) : p.hd <= 128 ? launch_attend<DTYPE, 128>(a, p, stream) : launch_attend<DTYPE, 256>(a, p, stream);
 }
 }  // namespace
 
