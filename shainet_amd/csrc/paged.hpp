@@ -30,11 +30,10 @@ struct MapArgs {
   int n_seqs, seq_pages, n_pages, shift;
   int *slots, *positions, *row_seqs;  // of the new rows in the entries' order; -1 from the last one to max_rows
   int max_rows;
-  int *scratch;                // map_scratch_ints()
+  int *scratch;                // a word, zero, which a launch leaves so
   int *error;                  // device-writable: set to kMapNoRoom or kMapBadEntry where nothing was changed
 };
 constexpr int kMapNoRoom = 3, kMapBadEntry = 4;
-size_t map_scratch_ints();
 hipError_t launch_page_map(const MapArgs &a, hipStream_t stream);
 // every length 0, every page free, page 0 to be taken first
 hipError_t launch_page_reset(int *lens, int n_seqs, int *free_pages, int *n_free, int n_pages, hipStream_t stream);

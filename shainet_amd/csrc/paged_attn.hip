@@ -23,6 +23,7 @@
 // keys' rows, a few neighbouring columns of each, transposed within the lane's registers.
 #include "paged.hpp"
 #include "lane_quarters.hpp"
+#include "lane_sums.hpp"
 #include "split_mfma.hpp"
 
 namespace shainet {
@@ -409,23 +410,6 @@ struct Wave {
     take<false>(tile, 0, 0);
   }
 };
-
-// Sum, or maximum (of numbers that are not negative), over the lanes up to this one.
-template <typename F>
-__device__ __forceinline__ int scan_lanes(int x, F two) {
-  x = two(x, __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false));  // row_shr 1, 2, 4, 8
-  x = two(x, __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false));
-  x = two(x, __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false));
-  x = two(x, __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false));
-  x = two(x, __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false));  // row_bcast 15, 31
-  return two(x, __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false));
-}
-__device__ __forceinline__ int sum_lanes(int x) {
-  return scan_lanes(x, [](int a, int b) { return a + b; });
-}
-__device__ __forceinline__ int max_lanes(int x) {
-  return scan_lanes(x, [](int a, int b) { return max(a, b); });
-}
 
 // How a launch shares out its work; the same for all workgroups, each of which makes it for itself.
 enum { kSpans, kChunks, kWavefronts };

@@ -26,7 +26,7 @@ struct shainet_paged_cache {
   char *k = nullptr, *v = nullptr;
   int *table = nullptr, *lens = nullptr, *free_pages = nullptr, *n_free = nullptr;
   int *pin = nullptr;      // [n_seqs + 1] on its way from the device
-  int *scratch = nullptr;  // map_scratch_ints()
+  int *scratch = nullptr;  // a word for maps
   void *workspace = nullptr;
   // steps: allocated with the cache, so that a step allocates nothing
   int *step_slots = nullptr, *step_positions = nullptr, *step_seqs = nullptr;  // [n_seqs]
@@ -249,7 +249,7 @@ int shainet_paged_cache_create(shainet_paged_cache **out, shainet_attn_ctx *ctx,
   if (e == hipSuccess) e = hipMalloc((void **)&pc->free_pages, (size_t)n_pages * sizeof(int));
   if (e == hipSuccess) e = hipMalloc((void **)&pc->n_free, sizeof(int));
   if (e == hipSuccess) e = hipHostMalloc((void **)&pc->pin, (n_seqs + 1) * sizeof(int), hipHostMallocDefault);
-  if (e == hipSuccess) e = hipMalloc((void **)&pc->scratch, map_scratch_ints() * sizeof(int));
+  if (e == hipSuccess) e = hipMalloc((void **)&pc->scratch, sizeof(int));
   if (e == hipSuccess) e = hipMalloc(&pc->workspace, ws);
   if (e == hipSuccess) e = hipMalloc((void **)&pc->step_slots, n_seqs * sizeof(int));
   if (e == hipSuccess) e = hipMalloc((void **)&pc->step_positions, n_seqs * sizeof(int));
@@ -259,6 +259,7 @@ int shainet_paged_cache_create(shainet_paged_cache **out, shainet_attn_ctx *ctx,
   if (e == hipSuccess) e = hipMemsetAsync(pc->v, 0, pool, ctx->stream);
   if (e == hipSuccess) e = hipMemsetAsync(pc->table, 0xff, table * sizeof(int), ctx->stream);
   if (e == hipSuccess) e = hipMemsetAsync(pc->workspace, 0, ws, ctx->stream);
+  if (e == hipSuccess) e = hipMemsetAsync(pc->scratch, 0, sizeof(int), ctx->stream);
   if (e == hipSuccess) e = launch_page_reset(pc->lens, n_seqs, pc->free_pages, pc->n_free, n_pages, ctx->stream);
   if (e == hipSuccess) e = hipStreamSynchronize(ctx->stream);
   if (e != hipSuccess && !rc) rc = hip_fail(e, "allocation of a cache in pages");
