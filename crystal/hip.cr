@@ -261,6 +261,61 @@ module SHAInet
       check fn.call(ctx, cache, n_seqs, q, k, v, out_ptr)
     end
 
+    # A cache in pages (device pointers but for paged_cache_read's and attn_forward_paged's lists): see the header.
+    PAGE_F32  = 0
+    PAGE_BF16 = 1
+    PAGE_F16  = 2
+
+    def paged_cache_create(ctx : Handle, layers : Int32, n_pages : Int32, page_rows : Int32, n_seqs : Int32,
+                           seq_pages : Int32, dtype : Int32 = PAGE_BF16) : Handle
+      fn = Proc(Pointer(Handle), Handle, Int32, Int32, Int32, Int32, Int32, Int32, Int32).new(sym("shainet_paged_cache_create"), Pointer(Void).null)
+      cache = Handle.null
+      status = fn.call(pointerof(cache), ctx, layers, n_pages, page_rows, n_seqs, seq_pages, dtype)
+      if status == 3
+        GC.collect
+        status = fn.call(pointerof(cache), ctx, layers, n_pages, page_rows, n_seqs, seq_pages, dtype)
+      end
+      check(status)
+      cache
+    end
+
+    def paged_cache_destroy(cache : Handle)
+      Proc(Handle, Int32).new(sym("shainet_paged_cache_destroy"), Pointer(Void).null).call(cache)
+    end
+
+    def paged_cache_len(cache : Handle, seq : Int32 = 0) : Int32
+      Proc(Handle, Int32, Int32).new(sym("shainet_paged_cache_len"), Pointer(Void).null).call(cache, seq)
+    end
+
+    def paged_cache_free_pages(cache : Handle) : Int32
+      Proc(Handle, Int32).new(sym("shainet_paged_cache_free_pages"), Pointer(Void).null).call(cache)
+    end
+
+    def paged_cache_clear(cache : Handle, seq : Int32 = -1)
+      check Proc(Handle, Int32, Int32).new(sym("shainet_paged_cache_clear"), Pointer(Void).null).call(cache, seq)
+    end
+
+    def paged_cache_truncate(cache : Handle, seq : Int32, len : Int32)
+      check Proc(Handle, Int32, Int32, Int32).new(sym("shainet_paged_cache_truncate"), Pointer(Void).null).call(cache, seq, len)
+    end
+
+    def paged_cache_lengths_from_device(cache : Handle)
+      check Proc(Handle, Int32).new(sym("shainet_paged_cache_lengths_from_device"), Pointer(Void).null).call(cache)
+    end
+
+    def attn_step_paged(ctx : Handle, cache : Handle, layer : Int32, seq_ids : Pointer(Int32), n : Int32,
+                        q : Pointer(Float32), k : Pointer(Float32), v : Pointer(Float32), out_ptr : Pointer(Float32))
+      fn = Proc(Handle, Handle, Int32, Pointer(Int32), Int32, Pointer(Float32), Pointer(Float32), Pointer(Float32), Pointer(Float32), Int32).new(sym("shainet_attn_step_paged"), Pointer(Void).null)
+      check fn.call(ctx, cache, layer, seq_ids, n, q, k, v, out_ptr)
+    end
+
+    # Host-pointer mode, any number of new rows for each of several sequences.
+    def attn_forward_paged(ctx : Handle, cache : Handle, layer : Int32, seq_ids : Array(Int32), new_tokens : Array(Int32),
+                           q : Pointer(Float32), k : Pointer(Float32), v : Pointer(Float32), out_ptr : Pointer(Float32))
+      fn = Proc(Handle, Handle, Int32, Pointer(Int32), Pointer(Int32), Int32, Pointer(Float32), Pointer(Float32), Pointer(Float32), Pointer(Float32), Int32, Int32).new(sym("shainet_attn_forward_paged"), Pointer(Void).null)
+      check fn.call(ctx, cache, layer, seq_ids.to_unsafe, new_tokens.to_unsafe, new_tokens.size, q, k, v, out_ptr, MEM_HOST)
+    end
+
     def attn_sync(ctx : Handle)
       check Proc(Handle, Int32).new(sym("shainet_attn_sync"), Pointer(Void).null).call(ctx)
     end

@@ -50,10 +50,15 @@ module SHAInet
     def kv_cache_destroy(*args)
     end
 
+    def paged_cache_destroy(*args)
+    end
+
     {% for name in %w(sym malloc memcpy kv_cache_append_f32 attention_kv_f32 attn_create attn_set_bias
                      kv_cache_create kv_cache_clear kv_cache_len kv_cache_capacity kv_cache_reserve
                      attn_forward attn_forward_noalloc attn_decode_step kv_cache_lengths_to_device
-                     kv_cache_lengths_from_device attn_sync rope_apply matmul_f32 check) %}
+                     kv_cache_lengths_from_device attn_sync rope_apply matmul_f32 check paged_cache_create paged_cache_len
+                     paged_cache_free_pages paged_cache_clear paged_cache_truncate paged_cache_lengths_from_device
+                     attn_step_paged attn_forward_paged) %}
       def {{name.id}}(*args)
         raise "HIP disabled"
       end

@@ -273,7 +273,7 @@ int shainet_attn_append_paged(shainet_attn_ctx *ctx, shainet_paged_cache *cache,
 /* Grouped-query attention of row r (rotated queries, 1/sqrt(head_dim) applied here) over the first positions[r] + 1 rows of
  * sequence row_seqs[r], by the table (the lengths are not looked at; several rows may name one sequence).  A row with
  * row_seqs outside 0..n_seqs-1 leaves its output alone; one with positions < 0, or whose keys' pages are all outside the
- * pool, gets zeros.  At most SHAINET_HIP_MAX_PAGED_SEQS rows.  Rows of q_rot and out at the given strides.  Asynchronous on the
+ * pool, gets zeros.  At most SHAINET_HIP_MAX_PAGED_SEQS rows, and rows * seq_pages * page_rows below 2^34.  Rows of q_rot and out at the given strides.  Asynchronous on the
  * context's stream.  Scores, softmax and sums are float32; the keys and values of the pages' numbers as
  * they are.  Replays of recordings that use one cache must not overlap. */
 int shainet_attn_attend_paged(shainet_attn_ctx *ctx, shainet_paged_cache *cache, int layer, const int *row_seqs,
@@ -281,15 +281,16 @@ int shainet_attn_attend_paged(shainet_attn_ctx *ctx, shainet_paged_cache *cache,
                               long long out_stride);
 /* A decode step: one new row for each of n sequences (seq_ids: device array, null: sequences 0..n-1); map, append and attend
  * with lists of the cache's own.  q [n, num_heads*head_dim], k, v [n, num_kv_heads*head_dim], out like q, device pointers.
- * Layer 0 maps the rows; calls for the layers behind it use that map.  Can be recorded and replayed.  A step that found no
- * room leaves `out` alone (see map_rows). */
+ * Layer 0 maps the rows; calls for the layers behind it use that map (refused once lengths were changed otherwise).  Can be
+ * recorded and replayed.  A step that found no room leaves `out` alone (see map_rows). */
 int shainet_attn_step_paged(shainet_attn_ctx *ctx, shainet_paged_cache *cache, int layer, const int *seq_ids, int n,
                             const float *q, const float *k, const float *v, float *out);
 /* shainet_attn_forward over a cache in pages: any number of new rows for each of up to SHAINET_HIP_MAX_BATCH sequences (host
  * arrays seq_ids and new_tokens), planned on the host, which must know the lengths.  Sequences with more than a few new rows
  * have their pages gathered into one piece of float32 scratch (which grows on demand) first and run as any prompt does.  Layer 0 maps and counts
- * the rows; calls for the layers behind it give the same seq_ids and new_tokens.  SHAINET_HIP_ERR_CAPACITY, and
- * nothing appended, when a sequence would outgrow its table or the pages do not suffice. */
+ * the rows; calls for the layers behind it give the same seq_ids and new_tokens.  Not to be recorded: the lengths are part of
+ * the plan.  SHAINET_HIP_ERR_CAPACITY, and nothing appended, when a sequence would outgrow its table or the pages do not
+ * suffice. */
 int shainet_attn_forward_paged(shainet_attn_ctx *ctx, shainet_paged_cache *cache, int layer, const int *seq_ids,
                                const int *new_tokens, int n_seqs, const float *q, const float *k, const float *v,
                                float *out, int mem);

@@ -50,7 +50,7 @@ struct PagedAttendArgs {
   float *out;
   long long q_stride, out_stride;
   const int *row_seqs, *positions;
-  int rows, H;
+  int rows, H, g;              // g: query heads per kv head
   float scale;
   void *workspace;             // paged_attend_workspace() bytes, zero when allocated; a launch leaves its counts zero
 };

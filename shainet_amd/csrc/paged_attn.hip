@@ -411,6 +411,10 @@ struct Wave {
   }
 };
 
+// a / b of whole numbers, a below 2^53: the rounded quotient is off by at most 2^-53 a / b, less than the 1 / b that parts a
+// quotient from the next whole number above.  (A division of 64-bit integers is over a hundred instructions.)
+__device__ __forceinline__ int quotient(long long a, long long b) { return (int)((double)a / (double)b); }
+
 // How a launch shares out its work; the same for all workgroups, each of which makes it for itself.
 enum { kSpans, kChunks, kWavefronts };
 
@@ -431,9 +435,9 @@ __global__ __launch_bounds__((64 * Tile<DTYPE, HD>::WAVES), (Tile<DTYPE, HD>::WA
   // (values from LDS that are the same in all lanes are said to be: they live in scalar registers then)
   auto same = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
   const int hd = PAD ? p.hd : HD;
-  const int g = a.H / p.KV, per_kv = (g + kCols - 1) / kCols, pairs = p.KV * per_kv;
+  const int g = a.g, per_kv = (g + kCols - 1) / kCols, pairs = p.KV * per_kv;
   const int most_keys = (int)min((long long)p.seq_pages << p.shift, 0x3fffffffLL);
-  const int wgs = (int)gridDim.x;
+  constexpr int wgs = 256 * T::PER_CU;  // of every launch
 
   // rows of a length that has a sequence; -1: a row to be left alone
   auto length_of = [&](int r, int &seq) {
@@ -496,12 +500,12 @@ __global__ __launch_bounds__((64 * Tile<DTYPE, HD>::WAVES), (Tile<DTYPE, HD>::WA
   } else if (unit < kShortSpan && n_pairs <= wgs) {
     // chunks of pairs, one a workgroup: sum of ceil(tiles / unit) <= total / unit + pairs
     mode = kChunks;
-    unit = n_pairs < wgs && most > T::WHOLE ? max((total + (wgs - n_pairs) - 1) / (wgs - n_pairs), (long long)WAVES) : most;
+    unit = n_pairs < wgs && most > T::WHOLE ? max((long long)quotient(total + (wgs - n_pairs) - 1, wgs - n_pairs), (long long)WAVES) : most;
   }
   if (mode != kWavefronts) {  // units of one kv head before each row
     auto units_of = [&](int r) {
       const int tiles = tiles_of(known_length(r));
-      return mode == kSpans ? tiles : (tiles + (int)unit - 1) / (int)unit;
+      return mode == kSpans ? tiles : quotient(tiles + unit - 1, unit);
     };
     if (few) {
       const int mine = lane < a.rows ? units_of(lane) : 0, upto = sum_lanes(mine);
@@ -552,7 +556,7 @@ __global__ __launch_bounds__((64 * Tile<DTYPE, HD>::WAVES), (Tile<DTYPE, HD>::WA
   auto next_segment = [&](Segment &s) {
     while (at < end) {
       if (mode == kWavefronts) {
-        row = (int)(at / pairs);
+        row = quotient(at, pairs);
         s.pair = (int)(at - (long long)row * pairs);
         at += (long long)wgs * WAVES;
       } else {
@@ -576,20 +580,20 @@ __global__ __launch_bounds__((64 * Tile<DTYPE, HD>::WAVES), (Tile<DTYPE, HD>::WA
       }
       const int units = same(starts[row + 1] - starts[row]);
       const long long of_row = (long long)same(starts[row]) * pairs;
-      s.pair = same((int)((at - of_row) / units));
+      s.pair = same(quotient(at - of_row, units));
       const long long begins = of_row + (long long)s.pair * units;
       const int from = (int)(at - begins);
       if (mode == kSpans) {
         s.first = from;
         s.last = (int)(min(end, begins + units) - begins);
         at += s.last - s.first;
-        s.first_wg = (int)(begins / unit);
-        s.last_wg = (int)((begins + units - 1) / unit);
+        s.first_wg = quotient(begins, unit);
+        s.last_wg = quotient(begins + units - 1, unit);
         s.late = begins > blockIdx.x * unit;
         s.first_late = begins > s.first_wg * unit;
       } else {  // equal shares
-        s.first = (int)((long long)tiles * from / units);
-        s.last = (int)((long long)tiles * (from + 1) / units);
+        s.first = quotient((long long)tiles * from, units);
+        s.last = quotient((long long)tiles * (from + 1), units);
         at += 1;
         s.first_wg = (int)begins;
         s.last_wg = (int)begins + units - 1;
@@ -610,13 +614,14 @@ __global__ __launch_bounds__((64 * Tile<DTYPE, HD>::WAVES), (Tile<DTYPE, HD>::WA
   const int step = alone ? 1 : WAVES, mine = alone ? 0 : wave;
   u32x4 *const queries = (u32x4 *)shared + (alone ? wave * (QUERIES / 4) : 0);
   w.q = queries;
-  auto head_of = [&](const Segment &s) { return s.pair / per_kv * g + s.pair % per_kv * kCols; };
-  auto cols_of = [&](const Segment &s) { return min(kCols, g - s.pair % per_kv * kCols); };
+  auto kv_of = [&](const Segment &s) { return per_kv == 1 ? s.pair : s.pair / per_kv; };
+  auto head_of = [&](const Segment &s) { return kv_of(s) * g + (s.pair - kv_of(s) * per_kv) * kCols; };
+  auto cols_of = [&](const Segment &s) { return min(kCols, g - (s.pair - kv_of(s) * per_kv) * kCols); };
   auto rows_of = [&](const Segment &s) { return a.q + s.row * a.q_stride + (long long)head_of(s) * hd; };
   typename Wave<DTYPE, HD, PAD>::Raw raw;
   // a segment's table entries and queries are asked for first, then its first tile
   auto start = [&](const Segment &s) {
-    w.start(s.seq, s.len, s.pair / per_kv, s.first + mine, step);
+    w.start(s.seq, s.len, kv_of(s), s.first + mine, step);
     if (!alone) w.ask_queries(raw, rows_of(s), cols_of(s), wave, WAVES);
     w.ask(s.first + mine, s.last);
   };
@@ -848,7 +853,7 @@ hipError_t launch_attend(const PagedAttendArgs &a, const PagePool &p, hipStream_
   constexpr int wgs = 256 * Tile<DTYPE, HD>::PER_CU;
   static_assert(wgs <= kMaxWorkgroups, "counts and parts");
   const auto kernel = p.hd == HD ? paged_attend_kernel<DTYPE, HD, false> : paged_attend_kernel<DTYPE, HD, true>;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)wgs), dim3(64 * Tile<DTYPE, HD>::WAVES), 0, stream, a, p);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)wgs), dim3(64 * Tile<DTYPE, HD>::WAVES), 0, stream, a, p);  // (the kernel counts on that many)
   return hipGetLastError();
 }
 template <int DTYPE>

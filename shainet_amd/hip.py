@@ -523,12 +523,13 @@ class AttnContext:
         """shainet_attn_append_paged: bias, QK-norm and rotation of rows of q, k and v (torch CUDA float32, rows may be
         strided); K and V rows into slots[row] of a `PagedKVCache`, rotated queries into q_rot.  slots and positions are
         int32 CUDA tensors, as `PagedKVCache.map_rows` writes them."""
-        rows = _ints(slots)
-        _ints(positions, rows)
-        qs, ks, vs = _rows(q, rows, self.q_dim), _rows(k, rows, self.kv_dim), _rows(v, rows, self.kv_dim)
+        dev = cache._device
+        rows = _ints(slots, dev)
+        _ints(positions, dev, rows)
+        qs, ks, vs = _rows(q, dev, rows, self.q_dim), _rows(k, dev, rows, self.kv_dim), _rows(v, dev, rows, self.kv_dim)
         if q_rot is None:
             q_rot = q.new_empty((rows, self.q_dim))
-        elif _rows(q_rot, rows, self.q_dim) != self.q_dim:
+        elif _rows(q_rot, dev, rows, self.q_dim) != self.q_dim:
             raise ArgumentError("q_rot must be contiguous")
         rc = _lib.shainet_attn_append_paged(self._h, cache._h, layer, slots.data_ptr(), positions.data_ptr(), rows, q.data_ptr(), qs,
                                             k.data_ptr(), ks, v.data_ptr(), vs, q_rot.data_ptr())
@@ -539,9 +540,10 @@ class AttnContext:
     def attend_paged(self, cache, row_seqs, positions, q_rot, out=None, layer=0):
         """shainet_attn_attend_paged: attention of rotated query rows over the first positions[row] + 1 rows of sequence
         row_seqs[row] of a `PagedKVCache` (int32 CUDA tensors).  Rows whose row_seqs is no sequence are left alone in `out`."""
-        rows = _ints(row_seqs)
-        _ints(positions, rows)
-        stride = _rows(q_rot, rows, self.q_dim)
+        dev = cache._device
+        rows = _ints(row_seqs, dev)
+        _ints(positions, dev, rows)
+        stride = _rows(q_rot, dev, rows, self.q_dim)
         if out is None:
             import torch
 
@@ -549,7 +551,7 @@ class AttnContext:
             if torch.cuda.current_stream().cuda_stream != (self.stream or 0):
                 torch.cuda.current_stream().synchronize()  # (the zeros of rows left alone are there before the kernel writes)
         rc = _lib.shainet_attn_attend_paged(self._h, cache._h, layer, row_seqs.data_ptr(), positions.data_ptr(), rows, q_rot.data_ptr(),
-                                            stride, out.data_ptr(), _rows(out, rows, self.q_dim))
+                                            stride, out.data_ptr(), _rows(out, dev, rows, self.q_dim))
         if rc:
             _check(rc)
         return out
@@ -557,10 +559,10 @@ class AttnContext:
     def step_paged(self, cache, q, k, v, out, seq_ids=None, layer=0):
         """shainet_attn_step_paged: one new row for each of q.shape[0] sequences of a `PagedKVCache` (seq_ids: int32 CUDA
         tensor; None: the first ones), mapped, placed and attended by launches that can be recorded and replayed."""
-        n, qd, kd = q.shape[0], self.q_dim, self.kv_dim
+        dev, n, qd, kd = cache._device, q.shape[0], self.q_dim, self.kv_dim
         if seq_ids is not None:
-            _ints(seq_ids, n)
-        if (_rows(q, n, qd), _rows(k, n, kd), _rows(v, n, kd), _rows(out, n, qd)) != (qd, kd, kd, qd):
+            _ints(seq_ids, dev, n)
+        if (_rows(q, dev, n, qd), _rows(k, dev, n, kd), _rows(v, dev, n, kd), _rows(out, dev, n, qd)) != (qd, kd, kd, qd):
             raise ArgumentError("q, k, v and out must be contiguous")
         rc = _lib.shainet_attn_step_paged(self._h, cache._h, layer, None if seq_ids is None else seq_ids.data_ptr(), n, q.data_ptr(),
                                           k.data_ptr(), v.data_ptr(), out.data_ptr())
@@ -588,38 +590,39 @@ class AttnContext:
 
             if out is None:
                 out = torch.empty_like(q)
+            dev = cache._device
             for t, width in ((q, self.q_dim), (k, self.kv_dim), (v, self.kv_dim), (out, self.q_dim)):
-                if _rows(t, rows, width) != width:
+                if _rows(t, dev, rows, width) != width:
                     raise ArgumentError("q, k, v and out must be contiguous")
             mem = MEM_DEVICE
         _check(lib().shainet_attn_forward_paged(self._h, cache._h, layer, ids, nt, n, _ptr(q), _ptr(k), _ptr(v), _ptr(out), mem))
         return out
 
 
-def _ints(t, n=None):
-    """Checks a CUDA int32 list (of n entries), as the calls on pages take them; returns its length."""
+def _ints(t, device, n=None):
+    """Checks an int32 list (of n entries) on a device, as the calls on pages take them; returns its length."""
     try:
         size = t.numel()
-        if t.dtype is _I32 and t.is_cuda and t.is_contiguous() and (n is None or n == size):
+        if t.dtype is _I32 and t.get_device() == device and t.is_contiguous() and (n is None or n == size):
             return size
-    except (AttributeError, TypeError):
+    except (AttributeError, TypeError, RuntimeError):
         pass
-    raise ArgumentError("expected a contiguous int32 CUDA tensor" + ("" if n is None else " of %d entries" % n))
+    raise ArgumentError("expected a contiguous int32 tensor%s on the cache's device" % ("" if n is None else " of %d entries" % n))
 
 
-def _rows(t, n, width):
-    """Checks n CUDA float32 rows of `width` neighbouring numbers; returns the distance of two rows."""
+def _rows(t, device, n, width):
+    """Checks n float32 rows of `width` neighbouring numbers on a device; returns the distance of two rows."""
     try:
-        if t.dtype is _F32 and t.is_cuda and t.shape == (n, width):
+        if t.dtype is _F32 and t.get_device() == device and t.shape == (n, width):
             far, near = t.stride()
             if near == 1 or width == 1:
                 if n < 2:
                     return width
                 if far >= width:
                     return far
-    except (AttributeError, TypeError):
+    except (AttributeError, TypeError, RuntimeError):
         pass
-    raise ArgumentError("expected a float32 CUDA tensor of %d rows of %d" % (n, width))
+    raise ArgumentError("expected a float32 tensor of %d rows of %d on the cache's device" % (n, width))
 
 
 class _PagedHandle:
@@ -658,6 +661,12 @@ class PagedKVCache:
         self.ctx = ctx
         self._handle = _PagedHandle(ctx, layers, n_pages, page_rows, n_seqs, seq_pages, self.DTYPES[dtype])
         self._h = self._handle.h
+        try:
+            import torch
+
+            self._device = torch.cuda.current_device()
+        except ImportError:  # (host arrays only)
+            self._device = None
         self.n_pages, self.page_rows, self.n_seqs, self.seq_pages, self.dtype, self.layers = n_pages, page_rows, n_seqs, seq_pages, dtype, layers
 
     def close(self):
@@ -693,18 +702,19 @@ class PagedKVCache:
     def map_rows(self, delta, slots=None, positions=None, row_seqs=None, seq_ids=None):
         """shainet_paged_cache_map_rows: sequences seq_ids (None: the first ones) change their lengths by delta rows; slots,
         positions and row_seqs of the rows gained.  int32 CUDA tensors; the three lists may be left out where no row is gained."""
-        n = _ints(delta)
+        dev = self._device
+        n = _ints(delta, dev)
         if seq_ids is not None:
-            _ints(seq_ids, n)
+            _ints(seq_ids, dev, n)
             seq_ids = seq_ids.data_ptr()
         if slots is None or positions is None or row_seqs is None:
             if not (slots is positions is row_seqs):
                 raise ArgumentError("slots, positions and row_seqs go together")
             rc = _lib.shainet_paged_cache_map_rows(self._h, seq_ids, delta.data_ptr(), n, None, None, None, 0)
         else:
-            most = _ints(slots)
-            _ints(positions, most)
-            _ints(row_seqs, most)
+            most = _ints(slots, dev)
+            _ints(positions, dev, most)
+            _ints(row_seqs, dev, most)
             rc = _lib.shainet_paged_cache_map_rows(self._h, seq_ids, delta.data_ptr(), n, slots.data_ptr(), positions.data_ptr(),
                                                    row_seqs.data_ptr(), most)
         if rc:

@@ -649,3 +649,129 @@ def test_a_table_of_angles_is_not_extended_while_recording(hip, torch):
     ctx.step_paged(cache, *x, out)
     ctx.sync()
     assert torch.allclose(out, torch.ones_like(out))
+
+
+@pytest.mark.parametrize("dtype,P", [("bf16", 16), ("f32", 64), ("f16", 1024)])
+def test_pages_behind_four_gigabytes(hip, torch, dtype, P):
+    """Sequences in the last pages of pools of more than 2^32 bytes each, by every call."""
+    H, KV, hd = 8, 4, 128
+    rng = np.random.default_rng(6)
+    ctx = _ctx(hip, torch, H, KV, hd)
+    page = KV * P * hd * (4 if dtype == "f32" else 2)
+    n_pages = (2 ** 32 + 2 ** 26) // page
+    cache = hip.PagedKVCache(ctx, n_pages, P, 2, 40, dtype=dtype)
+    cache.free_pages.copy_(torch.arange(n_pages, dtype=torch.int32, device="cuda"))  # the last page goes first
+    plain = hip.KVCache(ctx, 2, 600)
+    worst = 0.0
+    for new, ids in (([400, 33], [0, 1]), ([1, 9], [1, 0]), ([1], [0])):
+        rows = [torch.from_numpy(rng.standard_normal((sum(new), w * hd)).astype(np.float32)).cuda() for w in (H, KV, KV)]
+        got = ctx.forward_paged(cache, *rows, new, seq_ids=ids)
+        want = ctx.forward(plain, *rows, new, seq_ids=ids)
+        ctx.sync()
+        worst = max(worst, (got - want).abs().max().item())
+    assert (cache.table[0, :pages_of(400, P)] >= n_pages - 40).all() and cache.table[0, 0].item() == n_pages - 1
+    assert worst <= _tolerance(dtype)
+    rows = [torch.from_numpy(rng.standard_normal((2, w * hd)).astype(np.float32)).cuda() for w in (H, KV, KV)]
+    got = ctx.step_paged(cache, *rows, torch.empty_like(rows[0]))
+    want = ctx.forward(plain, *rows, [1, 1])
+    ctx.sync()
+    assert (got - want).abs().max().item() <= _tolerance(dtype)
+    cache.lengths_from_device()
+    for a, b in zip(cache.read(0, 3, 0, cache.len(0)), plain.read(0, 3, 0, plain.len(0))):
+        assert np.abs(a - b).max() <= (0 if dtype == "f32" else 2.0 ** -8 * np.abs(b).max())
+
+
+def test_other_layers_use_the_rows_of_layer_0_only(hip, torch):
+    H, KV, hd = 4, 2, 64
+    ctx = _ctx(hip, torch, H, KV, hd)
+    cache = hip.PagedKVCache(ctx, 20, 8, 3, 5, layers=2)
+    rows = lambda n: [torch.zeros((n, w * hd), device="cuda") for w in (H, KV, KV)]  # noqa: E731
+    lists = [torch.empty(3, dtype=torch.int32, device="cuda") for _ in range(3)]
+    out = torch.empty((2, H * hd), device="cuda")
+    steps = lambda layer: ctx.step_paged(cache, *rows(2), out, layer=layer)  # noqa: E731
+    forward = lambda layer: ctx.forward_paged(cache, *rows(3), [2, 1], seq_ids=[2, 0], layer=layer)  # noqa: E731
+    changes = (lambda: cache.map_rows(_ints(torch, [1]), *lists), lambda: cache.truncate(0, 0), lambda: cache.clear(),
+               lambda: cache.clear(0))
+    for change in changes:
+        for call, other in ((steps, forward), (forward, steps)):
+            cache.clear()
+            call(0)
+            call(1)
+            cache.lengths_from_device()
+            call(1)  # (nothing was changed)
+            change()
+            cache.lengths_from_device()
+            with pytest.raises(hip.ArgumentError, match="layer"):
+                call(1)
+            cache.clear()
+            call(0)
+            cache.lengths_from_device()
+            with pytest.raises(hip.ArgumentError, match="layer"):
+                other(1)
+    cache.clear()
+    steps(0)
+    with pytest.raises(hip.ArgumentError, match="layer"):
+        ctx.step_paged(cache, *rows(1), out[:1], layer=1)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_outputs_may_take_the_place_of_queries(hip, torch, dtype):
+    H, KV, hd, P = 20, 1, 96, 16
+    rng = np.random.default_rng(31)
+    ctx = _ctx(hip, torch, H, KV, hd)
+    lens = [9000, 3, 0, 700]
+    cache, held = _filled(hip, torch, ctx, lens, P, dtype, rng)
+    q = rng.standard_normal((4, H * hd)).astype(np.float32)
+    seqs, positions = list(range(4)), [n - 1 for n in lens]
+    t = torch.from_numpy(q).cuda()
+    ctx.attend_paged(cache, _ints(torch, seqs), _ints(torch, positions), t, out=t)
+    ctx.sync()
+    _check_rows(t.cpu().numpy(), q, held, seqs, positions, hd)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("what", ["q", "k", "v"])
+def test_what_is_no_number_stays_in_its_row(hip, torch, what, dtype):
+    """NaN in a query, or in a key or value that counts, makes NaN of the outputs it enters and of no others."""
+    H, KV, hd, P = 4, 2, 64, 16
+    rng = np.random.default_rng(2)
+    ctx = _ctx(hip, torch, H, KV, hd)
+    cache, held = _filled(hip, torch, ctx, [300, 300], P, dtype, rng)
+    q = torch.from_numpy(rng.standard_normal((2, H * hd)).astype(np.float32)).cuda()
+    args = _ints(torch, [0, 1]), _ints(torch, [299, 299])
+    before = ctx.attend_paged(cache, *args, q)
+    if what == "q":
+        q[0, 2 * hd + 5] = float("nan")     # query head 2
+        bad = torch.zeros_like(before, dtype=torch.bool)
+        bad[0, 2 * hd:3 * hd] = True
+    else:
+        page = cache.table[0, 3].item()
+        (cache.k if what == "k" else cache.v)[page, 1, 7, 9] = float("nan")  # kv head 1: query heads 2 and 3
+        bad = torch.zeros_like(before, dtype=torch.bool)
+        bad[0, 2 * hd:] = True
+        if what == "v":
+            bad[0] = False
+            bad[0, 2 * hd + 9] = bad[0, 3 * hd + 9] = True
+    after = ctx.attend_paged(cache, *args, q)
+    ctx.sync()
+    assert torch.equal(torch.isnan(after), bad)
+    assert torch.equal(after[~bad], before[~bad])
+
+
+def test_steps_on_another_stream(hip, torch):
+    """A context moved to another stream takes its cache along; rows made there are seen there."""
+    H, KV, hd = 4, 2, 64
+    rng = np.random.default_rng(9)
+    ctx = _ctx(hip, torch, H, KV, hd)
+    cache, plain = hip.PagedKVCache(ctx, 40, 8, 3, 10, dtype="f32"), hip.KVCache(ctx, 3, 80)
+    for turn in range(6):
+        stream = torch.cuda.Stream()
+        ctx.set_stream(stream.cuda_stream)
+        with torch.cuda.stream(stream):
+            rows = [torch.from_numpy(rng.standard_normal((3, w * hd)).astype(np.float32)).cuda(non_blocking=True) for w in (H, KV, KV)]
+            got = ctx.step_paged(cache, *rows, torch.empty_like(rows[0]))
+            want = ctx.forward(plain, *rows, [1, 1, 1])
+            assert (got - want).abs().max().item() <= 2e-5, turn
+    cache.lengths_from_device()
+    assert [cache.len(s) for s in range(3)] == [6, 6, 6]
+    ctx.set_stream(torch.cuda.current_stream().cuda_stream)

@@ -62,7 +62,7 @@ def test_lists_that_are_no_device_lists_are_refused(lib):
     import torch
 
     cache = hip.PagedKVCache.__new__(hip.PagedKVCache)
-    cache._h, cache._handle, cache._views, cache.ctx = None, None, {}, None
+    cache._h, cache._handle, cache._views, cache.ctx, cache._device = None, None, {}, None, 0
     for bad in (torch.zeros(3, dtype=torch.int32), np.zeros(3, np.int32), torch.zeros(3)):
         with pytest.raises(hip.ArgumentError):
             cache.map_rows(bad)
@@ -70,4 +70,4 @@ def test_lists_that_are_no_device_lists_are_refused(lib):
         cache.table
     for bad in (torch.zeros(2, 8), np.zeros((2, 8), np.float32)):
         with pytest.raises(hip.ArgumentError):
-            hip._rows(bad, 2, 8)
+            hip._rows(bad, 0, 2, 8)
