@@ -83,7 +83,6 @@ struct Tile {
   static constexpr int WORDS = VEC * E / 4;                // of 4 bytes, in one
   static constexpr int PARTS = DTYPE == kPageF32 ? 1 : DTYPE == kPageBf16 ? 3 : 2;  // of a float operand
   static constexpr int WAVES = 4;                          // of a workgroup
-  static constexpr int PER_CU = HD == 256 ? 1 : 2;         // workgroups of a compute unit
   static constexpr int WHOLE = 12;                                 // tiles of a pair that is not worth being cut
 };
 
@@ -418,8 +417,9 @@ __device__ __forceinline__ int quotient(long long a, long long b) { return (int)
 // How a launch shares out its work; the same for all workgroups, each of which makes it for itself.
 enum { kSpans, kChunks, kWavefronts };
 
-template <int DTYPE, int HD, bool PAD>
-__global__ __launch_bounds__((64 * Tile<DTYPE, HD>::WAVES), (Tile<DTYPE, HD>::WAVES / 4 * Tile<DTYPE, HD>::PER_CU)) void paged_attend_kernel(PagedAttendArgs a, PagePool p) {
+// PER_CU: workgroups of a compute unit, 1 or 2.
+template <int DTYPE, int HD, bool PAD, int PER_CU>
+__global__ __launch_bounds__((64 * Tile<DTYPE, HD>::WAVES), (Tile<DTYPE, HD>::WAVES / 4 * PER_CU)) void paged_attend_kernel(PagedAttendArgs a, PagePool p) {
   using T = Tile<DTYPE, HD>;
   constexpr int WAVES = T::WAVES, THREADS = 64 * WAVES, STRIDE = HD + 4;
   constexpr int NEAR = 512;                                 // rows whose lengths stay at hand
@@ -437,7 +437,7 @@ __global__ __launch_bounds__((64 * Tile<DTYPE, HD>::WAVES), (Tile<DTYPE, HD>::WA
   const int hd = PAD ? p.hd : HD;
   const int g = a.g, per_kv = (g + kCols - 1) / kCols, pairs = p.KV * per_kv;
   const int most_keys = (int)min((long long)p.seq_pages << p.shift, 0x3fffffffLL);
-  constexpr int wgs = 256 * T::PER_CU;  // of every launch
+  constexpr int wgs = 256 * PER_CU;  // of every launch
 
   // rows of a length that has a sequence; -1: a row to be left alone
   auto length_of = [&](int r, int &seq) {
@@ -608,7 +608,7 @@ __global__ __launch_bounds__((64 * Tile<DTYPE, HD>::WAVES), (Tile<DTYPE, HD>::WA
   // 77 to 100 us and the others at 108 to 118 (16 sequences of 2048 to 8192 keys, float32).  The others' instructions go
   // first, therefore: half to one per cent of most launches.  (Spans of unequal lengths, or short ones for whoever is
   // ready, cost more in parts of pairs than they gave: 110 -> 113 and 121 us.)
-  if (T::PER_CU == 2 && (int)blockIdx.x >= wgs / 2) __builtin_amdgcn_s_setprio(3);
+  if (PER_CU == 2 && (int)blockIdx.x >= wgs / 2) __builtin_amdgcn_s_setprio(3);
   Wave<DTYPE, HD, PAD> w(p, a.scale);
   const bool alone = mode == kWavefronts;
   const int step = alone ? 1 : WAVES, mine = alone ? 0 : wave;
@@ -848,13 +848,26 @@ size_t paged_attend_workspace(int hd) {
 }
 
 namespace {
+template <int DTYPE, int HD, bool PAD, int PER_CU>
+hipError_t launch_attend(const PagedAttendArgs &a, const PagePool &p, hipStream_t stream) {
+  constexpr int wgs = 256 * PER_CU;  // (the kernel counts on that many)
+  static_assert(wgs <= kMaxWorkgroups, "counts and parts");
+  hipLaunchKernelGGL((paged_attend_kernel<DTYPE, HD, PAD, PER_CU>), dim3((unsigned)wgs), dim3(64 * Tile<DTYPE, HD>::WAVES), 0, stream, a, p);
+  return hipGetLastError();
+}
+// One workgroup on a compute unit reads long stretches of few pairs faster than two, of which the first gets ahead: 16 sequences of 2048 to
+// 8192 keys (128 pairs, float32) 106 us | two 109, one of 131072 (4 pairs, bfloat16) 50 | 53, 24 of 20 to 700 (192 pairs) 10.2 | 11.9.
+// Where there are more pairs than compute units two hide each other's beginnings and ends: 64 sequences of 100 to
+// 300 keys (512 pairs) 29 | 15 us, 77 of up to 5000 (308 pairs) 81 | 72.
 template <int DTYPE, int HD>
 hipError_t launch_attend(const PagedAttendArgs &a, const PagePool &p, hipStream_t stream) {
-  constexpr int wgs = 256 * Tile<DTYPE, HD>::PER_CU;
-  static_assert(wgs <= kMaxWorkgroups, "counts and parts");
-  const auto kernel = p.hd == HD ? paged_attend_kernel<DTYPE, HD, false> : paged_attend_kernel<DTYPE, HD, true>;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)wgs), dim3(64 * Tile<DTYPE, HD>::WAVES), 0, stream, a, p);  // (the kernel counts on that many)
-  return hipGetLastError();
+  if constexpr (HD == 256) {  // (registers for one)
+    return p.hd == HD ? launch_attend<DTYPE, HD, false, 1>(a, p, stream) : launch_attend<DTYPE, HD, true, 1>(a, p, stream);
+  } else {
+    if (p.hd != HD) return launch_attend<DTYPE, HD, true, 2>(a, p, stream);
+    const long long pairs = (long long)a.rows * p.KV * ((a.g + kCols - 1) / kCols);
+    return pairs <= 256 ? launch_attend<DTYPE, HD, false, 1>(a, p, stream) : launch_attend<DTYPE, HD, false, 2>(a, p, stream);
+  }
 }
 template <int DTYPE>
 hipError_t launch_attend(const PagedAttendArgs &a, const PagePool &p, hipStream_t stream) {
