@@ -211,8 +211,8 @@ int shainet_attn_decode_step(shainet_attn_ctx *ctx, shainet_kv_cache *cache, int
  * shainet_kv_cache reserves its capacity for every sequence ahead.  Here sequences take pages of page_rows rows
  * as they grow and give them back as they shrink, so that a server's memory holds as many rows as its requests
  * have.  For each of `layers` layers K and V are [n_pages][num_kv_heads][page_rows][head_dim] of float32, bfloat16
- * or float16 numbers (rows are rounded once, when they are placed; queries, sums and outputs are float32), and
- * all layers share, on the device,
+ * or float16 numbers (rows are rounded once, when they are placed; beyond 65504 float16 is infinite; queries, sums and outputs are
+ * float32), and all layers share, on the device,
  *   table [n_seqs][seq_pages]   the page of each page_rows rows of a sequence; entries behind its last page: anything
  *   lens [n_seqs]               rows of each sequence
  *   free_pages [n_pages]        a stack: its first *n_free entries are the pages that nobody holds
@@ -222,8 +222,9 @@ int shainet_attn_decode_step(shainet_attn_ctx *ctx, shainet_kv_cache *cache, int
  * n_pages * page_rows, n_seqs * seq_pages below 2^31, seq_pages * page_rows below 2^30.  The context gives the head
  * geometry and the stream and must outlive the cache; contexts of other layers may use the cache too, with
  * the same kv heads and head_dim, at most as many query heads, and the same stream (shainet_attn_set_stream).
- * Calls that rotate rows extend their context's cos/sin table to seq_pages * page_rows positions the first time, which waits
- * and cannot be recorded (SHAINET_HIP_ERR_ARGUMENT then); otherwise calls allocate nothing unless they say so.  Calls are made
+ * Calls that rotate rows extend their context's cos/sin table the first time, to as many positions as a sequence can have rows
+ * (append_paged: to seq_pages * page_rows, whatever the number of pages), up to 8 GiB of it; that cannot be recorded
+ * (SHAINET_HIP_ERR_ARGUMENT then).  Otherwise calls allocate nothing unless they say so.  Calls are made
  * with the device current that was current at creation.  One caller at a time per cache. */
 #define SHAINET_HIP_PAGE_F32 0
 #define SHAINET_HIP_PAGE_BF16 1
@@ -244,14 +245,17 @@ int shainet_paged_cache_arrays(shainet_paged_cache *cache, int layer, void **k, 
  * and given back, and for each row gained, in the entries' order, slots[r] = page * page_rows + row in the page,
  * positions[r] and row_seqs[r] are written (device arrays of max_rows entries; those behind the last row become -1).
  * Pages given back in a call can be taken in it; a call followed by its inverse leaves the stack as it was.
- * Asynchronous on the context's stream, depends on nothing but its arguments: can be recorded and replayed.  All or nothing: a sequence out of range or named twice, a length below 0, or too few pages, too
- * narrow a table or too many rows for the lists leave lengths, table and stack as they were and all three lists at -1;
- * the next shainet_attn_sync or shainet_paged_cache_lengths_from_device then returns SHAINET_HIP_ERR_ARGUMENT or
- * SHAINET_HIP_ERR_CAPACITY. */
+ * Asynchronous on the context's stream, depends on nothing but its arguments: can be recorded and replayed, as append_paged,
+ * attend_paged and step_paged can; the other calls are refused while the stream is recorded.  All or nothing: a sequence
+ * out of range or named twice, a length below 0, or too few pages, too narrow a table or too many rows for the lists leave
+ * lengths, table and stack as they were and all three lists at -1; the next shainet_attn_sync or
+ * shainet_paged_cache_lengths_from_device then returns SHAINET_HIP_ERR_ARGUMENT or SHAINET_HIP_ERR_CAPACITY. */
 int shainet_paged_cache_map_rows(shainet_paged_cache *cache, const int *seq_ids, const int *delta, int n, int *slots,
                                  int *positions, int *row_seqs, int max_rows);
-/* After calls that change lengths on the device (map_rows, step_paged, or replays of them) the host's copy is stale and
- * shainet_attn_forward_paged, truncate, read and the two calls for numbers are refused (-1) until this one, which waits. */
+/* After calls that change lengths on the device (map_rows, step_paged) the host's copy is stale and shainet_attn_forward_paged,
+ * truncate, read and the two calls for numbers are refused (-1) until this one, which waits.  A replay of such a call is not seen
+ * by the host: this one comes after it, too.  (Without it, truncate and forward_paged change nothing, and the next call that
+ * waits returns SHAINET_HIP_ERR_ARGUMENT.) */
 int shainet_paged_cache_lengths_from_device(shainet_paged_cache *cache);
 int shainet_paged_cache_len(const shainet_paged_cache *cache, int seq);
 int shainet_paged_cache_free_pages(const shainet_paged_cache *cache);
@@ -273,9 +277,10 @@ int shainet_attn_append_paged(shainet_attn_ctx *ctx, shainet_paged_cache *cache,
 /* Grouped-query attention of row r (rotated queries, 1/sqrt(head_dim) applied here) over the first positions[r] + 1 rows of
  * sequence row_seqs[r], by the table (the lengths are not looked at; several rows may name one sequence).  A row with
  * row_seqs outside 0..n_seqs-1 leaves its output alone; one with positions < 0, or whose keys' pages are all outside the
- * pool, gets zeros.  At most SHAINET_HIP_MAX_PAGED_SEQS rows, and rows * seq_pages * page_rows below 2^34.  Rows of q_rot and out at the given strides.  Asynchronous on the
- * context's stream.  Scores, softmax and sums are float32; the keys and values of the pages' numbers as
- * they are.  Replays of recordings that use one cache must not overlap. */
+ * pool, gets zeros; one that sees an infinite number or none gets outputs that are infinite or no numbers.  At most
+ * SHAINET_HIP_MAX_PAGED_SEQS rows, and rows * seq_pages * page_rows below 2^34.  Rows of q_rot and out at the given strides; out
+ * may be q_rot.  Asynchronous on the context's stream.  Scores, softmax and sums are float32, keys and values the pages'
+ * numbers as they are.  Replays of recordings that use one cache must not overlap. */
 int shainet_attn_attend_paged(shainet_attn_ctx *ctx, shainet_paged_cache *cache, int layer, const int *row_seqs,
                               const int *positions, int rows, const float *q_rot, long long q_stride, float *out,
                               long long out_stride);
@@ -287,8 +292,8 @@ int shainet_attn_step_paged(shainet_attn_ctx *ctx, shainet_paged_cache *cache, i
                             const float *q, const float *k, const float *v, float *out);
 /* shainet_attn_forward over a cache in pages: any number of new rows for each of up to SHAINET_HIP_MAX_BATCH sequences (host
  * arrays seq_ids and new_tokens), planned on the host, which must know the lengths.  Sequences with more than a few new rows
- * have their pages gathered into one piece of float32 scratch (which grows on demand) first and run as any prompt does.  Layer 0 maps and counts
- * the rows; calls for the layers behind it give the same seq_ids and new_tokens.  Not to be recorded: the lengths are part of
+ * have their pages gathered into one piece of float32 scratch (which grows on demand) first and run as any prompt does.  Layer 0
+ * maps and counts the rows; calls for the layers behind it give the same seq_ids and new_tokens.  Not to be recorded: the lengths are part of
  * the plan.  SHAINET_HIP_ERR_CAPACITY, and nothing appended, when a sequence would outgrow its table or the pages do not
  * suffice. */
 int shainet_attn_forward_paged(shainet_attn_ctx *ctx, shainet_paged_cache *cache, int layer, const int *seq_ids,

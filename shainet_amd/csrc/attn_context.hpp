@@ -50,6 +50,7 @@ struct shainet_attn_ctx {
   float *d_bq = nullptr, *d_bk = nullptr, *d_bv = nullptr;
   float2 *d_rope = nullptr;
   int rope_positions = 0;
+  std::vector<float2 *> old_rope;  // shorter tables, which recorded calls may still read
   hipStream_t stream = nullptr;      // where work is issued
   hipStream_t own_stream = nullptr;  // created with the context, destroyed with it
   shainet::DevBuf q_rot, partials, in_q, in_k, in_v, out;

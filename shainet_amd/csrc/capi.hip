@@ -61,8 +61,8 @@ int check_error_word(int *w) {
                 "lists hold: that call changed nothing, and its rows were neither placed nor attended");
   if (what == kMapBadEntry)
     return fail(SHAINET_HIP_ERR_ARGUMENT,
-                "a map of new rows found a sequence out of range or named twice, or a length below 0: that call changed nothing, "
-                "and its rows were neither placed nor attended");
+                "a map of new rows found a sequence out of range or named twice, a length below 0, or one that the host did not know "
+                "(shainet_paged_cache_lengths_from_device): that call changed nothing, and its rows were neither placed nor attended");
   if (what == 2)
     return fail(SHAINET_HIP_ERR_CAPACITY,
                 "a decode step found a sequence at the capacity of its cache or at the end of the context's "
@@ -173,7 +173,13 @@ int shainet::ensure_rope_table(shainet_attn_ctx *c, int positions) {
     c->rope_positions = want;
     return SHAINET_HIP_OK;
   }
-  std::vector<float2> tab((size_t)want * half);
+  std::vector<float2> tab;
+  try {
+    tab.resize((size_t)want * half);
+    c->old_rope.reserve(c->old_rope.size() + 1);
+  } catch (const std::bad_alloc &) {
+    return fail(SHAINET_HIP_ERR_ALLOC, "out of host memory for a cos/sin table of %d positions", want);
+  }
   for (int pos = 0; pos < want; ++pos)
     for (int i = 0; i < half; ++i) {
       if (c->rope_fp64) {
@@ -191,11 +197,8 @@ int shainet::ensure_rope_table(shainet_attn_ctx *c, int positions) {
     (void)hipFree(np);
     return hip_fail(e, "hipMemcpy(rope table)");
   }
-  if (c->d_rope) {
-    // kernels already queued may still read the old table
-    (void)hipStreamSynchronize(c->stream);
-    (void)hipFree(c->d_rope);
-  }
+  // kernels already queued and recorded calls still read the old table; together the old ones are no larger than the new one
+  if (c->d_rope) c->old_rope.push_back(c->d_rope);
   c->d_rope = np;
   c->rope_positions = want;
   return SHAINET_HIP_OK;
@@ -570,6 +573,7 @@ int shainet_attn_destroy(shainet_attn_ctx *c) {
   for (float *p : {c->d_q_norm, c->d_k_norm, c->d_bq, c->d_bk, c->d_bv})
     if (p) (void)hipFree(p);
   if (c->d_rope) (void)hipFree(c->d_rope);
+  for (float2 *p : c->old_rope) (void)hipFree(p);
   if (c->part_flag) (void)hipFree(c->part_flag);
   for (hipEvent_t ev : c->prof_events) (void)hipEventDestroy(ev);
   for (DevBuf *b : {&c->q_rot, &c->partials, &c->in_q, &c->in_k, &c->in_v, &c->out}) b->release();

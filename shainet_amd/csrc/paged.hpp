@@ -24,8 +24,8 @@ struct PagePool {
 struct MapArgs {
   int n;
   const int *ids, *delta;      // device; null: see `inlined`, else sequence i and one row
-  int inlined;                 // the two lists below instead, n <= kMaxSeqs
-  int id[kMaxSeqs], change[kMaxSeqs];
+  int inlined;                 // the lists below instead, n <= kMaxSeqs; a sequence whose length is not `was` is a bad entry
+  int id[kMaxSeqs], was[kMaxSeqs], change[kMaxSeqs];
   int *table, *lens, *free_pages, *n_free;
   int n_seqs, seq_pages, n_pages, shift;
   int *slots, *positions, *row_seqs;  // of the new rows in the entries' order; -1 from the last one to max_rows

@@ -5,12 +5,17 @@
 // pages' bytes bound it; a short one is bound by what a launch, the plan and a trip to memory take.
 //
 // Work split.  The key tiles (16 rows of float32, 32 of 16-bit numbers: 8 KiB of K and 8 of V at head_dim 128) of all
-// (row, kv head) pairs lie end to end and are cut into equal spans, one per workgroup, whatever the lengths; every workgroup
-// makes the sums that tell it where its span lies from the lengths themselves, so that nothing of a launch depends on them
-// but what it does, and a recorded one is good for any lengths.  The wavefronts of a workgroup take its tiles in turn, each with a
-// softmax of its own (running maximum, sum and output), and merge through LDS.  A pair that several workgroups share leaves
-// a part with each; the workgroup that adds its part last (a count per pair) adds them all up, in the order of the keys, so
-// results do not depend on who that is, and nobody waits for anybody.
+// (row, kv head) pairs lie end to end, each pair behind a few empty places for what it costs to begin one, and are cut into
+// equal spans, one per workgroup, whatever the lengths; every workgroup makes the sums that tell it where its span lies from the
+// lengths themselves, so that nothing of a launch depends on them but what it does, and a recorded one is good for any
+// lengths.  The wavefronts of a workgroup take its tiles in turn, each with a softmax of its own (running maximum, sum and
+// output), and merge through LDS.  A pair that several workgroups share leaves a part with each; the workgroup that adds its
+// part last (a count per pair) adds them all up, in the order of the keys, so results do not depend on who that is, and nobody
+// waits for anybody.  Short pairs are cut into chunks, one per workgroup, instead, and many short ones go to a wavefront each.
+//
+// Measured (shared rows of all: K and V of 8 kv heads of 128, 32 query heads, pages of 16): 64 sequences of 8192 to 32768 keys of bfloat16
+// 780 us, 6.7 TB/s (8 KiB pieces in any order, 64 KB on their way per compute unit, come at 6.5, 128 KB at 6.8); 16 of 2048 to 8192 of
+// float32 105 us, 6.2 TB/s; one sequence of 1024 (heads of 64) 9 us, of which an empty launch takes 4.
 //
 // A wavefront has one tile in registers: it asks for the next tile's K once the scores are made, and for its V once the outputs are,
 // straight from memory in the layout of the MFMA operands: for K 16 rows x 64 bytes per load, for V whole rows.  (Read
@@ -66,16 +71,24 @@ __device__ __forceinline__ f32x4 coherent_load4(const float *p) {
 constexpr int kCols = 16;  // query heads of a pair, at most: a larger group is several pairs
 constexpr int kMaxWorkgroups = 512;
 constexpr int kTickets = 4 * kMaxWorkgroups;  // two places a workgroup, two levels
+// Parts that are added up at once: a sequence of 1024 keys, whose 16 parts then take one round, 8.9 us | 11.3 by 8; 32 is as good.
 constexpr int kTeam = 16;
-constexpr int kShortSpan = 32, kWavefrontTiles = 8;
+// Pairs of which each workgroup would have less than this many tiles are cut into chunks, if there are no more of them than workgroups: 24
+// sequences of 20 to 700 keys (bfloat16) 10.5 us | as spans 15.6; 16 of 500 (float32), 16 tiles each, as spans 19 | as chunks 23.
+constexpr int kShortSpan = 16;
+// Pairs of up to this many, if there are more of them than workgroups, go to a wavefront each: 160 sequences of 50 to 480 keys, 8 kv heads
+// (bfloat16), 41 us | as spans 55; of 100 to 960, 30 tiles, 80 | 82, and 100 of those 53 | 60 but 75 | 72 where all are long.
+constexpr int kWavefrontTiles = 16;
+// Tiles that the beginning of a pair costs a workgroup: 39 sequences of up to 5000 keys (bfloat16) 64 us | 86 with none; with 8, 65.  Where all
+// are as long it costs a little: 16 of 500 (float32) 19 us | 17.8.
+constexpr int kBegin = 4;
 
 // What is laid out how for pages of a type and heads of up to HD.
 template <int DTYPE, int HD>
 struct Tile {
   static constexpr int E = DTYPE == kPageF32 ? 4 : 2;      // bytes of a number
-  static constexpr int S = DTYPE == kPageF32 ? 1 : 2;      // sixteens of keys of a block
-  static constexpr int BLOCKS = 1;                         // of a tile
-  static constexpr int BLOCK_KEYS = 16 * S, KEYS = BLOCKS * BLOCK_KEYS;
+  static constexpr int S = DTYPE == kPageF32 ? 1 : 2;      // sixteens of keys of a tile
+  static constexpr int KEYS = 16 * S;
   static constexpr int CHUNKS = HD * E / 64;               // 16-byte pieces of a K row per lane
   static constexpr int PER = 16 / E;                       // numbers in one
   static constexpr int VEC = HD == 96 ? 3 * PER / 4 : HD / 16 < PER ? HD / 16 : PER;  // neighbouring columns of a V row per lane
@@ -83,7 +96,8 @@ struct Tile {
   static constexpr int WORDS = VEC * E / 4;                // of 4 bytes, in one
   static constexpr int PARTS = DTYPE == kPageF32 ? 1 : DTYPE == kPageBf16 ? 3 : 2;  // of a float operand
   static constexpr int WAVES = 4;                          // of a workgroup
-  static constexpr int WHOLE = 12;                                 // tiles of a pair that is not worth being cut
+  // Tiles of a pair that is not worth being cut: one sequence of 100 keys (7 tiles of float32) 6.7 us | cut 8.4.
+  static constexpr int WHOLE = 12;
 };
 
 template <int WORDS>
@@ -109,9 +123,9 @@ struct Wave {
 
   // A tile in registers, or on its way there.
   struct Held {
-    u32x4 k[T::BLOCKS][T::S][T::CHUNKS];
-    VWords v[T::BLOCKS][KEYS_EACH][T::PIECES];
-    bool in[T::BLOCKS];  // whether this lane's V rows, which are the keys of its scores, lie in the pool
+    u32x4 k[T::S][T::CHUNKS];
+    VWords v[KEYS_EACH][T::PIECES];
+    bool in;  // whether this lane's V rows, which are the keys of its scores, lie in the pool
   };
   // This wavefront's share of a row of queries: chunks `first`, first + step, ...
   static constexpr int SHARE = (T::CHUNKS + T::WAVES - 1) / T::WAVES;
@@ -129,7 +143,7 @@ struct Wave {
   float c;         // scores to log2 units
   int down;        // float16: the queries were multiplied by 2^down
   struct Pages {
-    int k[T::BLOCKS], v[T::BLOCKS];  // of this lane's K row and V rows in a tile
+    int k, v;  // of this lane's K row and V rows in a tile
   };
   Pages now, next;  // of a walk's first tile, and of the tile to be asked for next
   const int *table;
@@ -141,12 +155,9 @@ struct Wave {
 
   // (behind the last tile: its last page again)
   __device__ __forceinline__ void look_up(Pages &at_page, int tile) const {
-#pragma unroll
-    for (int b = 0; b < T::BLOCKS; ++b) {
-      const int k0 = tile * T::KEYS + b * T::BLOCK_KEYS;
-      at_page.k[b] = table[min((k0 + (m >> 2) * KEYS_EACH) >> p.shift, last_page)];
-      at_page.v[b] = table[min((k0 + j * KEYS_EACH) >> p.shift, last_page)];
-    }
+    const int k0 = tile * T::KEYS;
+    at_page.k = table[min((k0 + (m >> 2) * KEYS_EACH) >> p.shift, last_page)];
+    at_page.v = table[min((k0 + j * KEYS_EACH) >> p.shift, last_page)];
   }
   __device__ __forceinline__ const char *row_at(const char *base, int page, int key) const {
     const long long row = ((long long)((unsigned)page < (unsigned)p.n_pages ? page : 0) * p.KV << p.shift) + (key & ((1 << p.shift) - 1));
@@ -161,33 +172,28 @@ struct Wave {
   __device__ __forceinline__ void ask_k(const Pages &at_page, int tile) {
     const int bytes = row_bytes();
 #pragma unroll
-    for (int b = 0; b < T::BLOCKS; ++b)
+    for (int s = 0; s < T::S; ++s) {
+      const char *row = row_at(k_base, at_page.k, tile * T::KEYS + (m >> 2) * KEYS_EACH + 4 * s + (m & 3));
 #pragma unroll
-      for (int s = 0; s < T::S; ++s) {
-        const char *row = row_at(k_base, at_page.k[b], tile * T::KEYS + b * T::BLOCK_KEYS + (m >> 2) * KEYS_EACH + 4 * s + (m & 3));
-#pragma unroll
-        for (int u = 0; u < T::CHUNKS; ++u) {
-          int at = (u * 4 + j) * 16;
-          if (PAD) at = at < bytes ? at : 0;
-          held.k[b][s][u] = __builtin_nontemporal_load((const u32x4 *)(row + at));
-        }
+      for (int u = 0; u < T::CHUNKS; ++u) {
+        int at = (u * 4 + j) * 16;
+        if (PAD) at = at < bytes ? at : 0;
+        held.k[s][u] = __builtin_nontemporal_load((const u32x4 *)(row + at));
       }
+    }
   }
   __device__ __forceinline__ void ask_v(const Pages &at_page, int tile) {
     const int bytes = row_bytes();
+    const char *row = row_at(v_base, at_page.v, tile * T::KEYS + j * KEYS_EACH);
+    held.in = (unsigned)at_page.v < (unsigned)p.n_pages;
 #pragma unroll
-    for (int b = 0; b < T::BLOCKS; ++b) {
-      const char *row = row_at(v_base, at_page.v[b], tile * T::KEYS + b * T::BLOCK_KEYS + j * KEYS_EACH);
-      held.in[b] = (unsigned)at_page.v[b] < (unsigned)p.n_pages;
+    for (int r = 0; r < KEYS_EACH; ++r)
 #pragma unroll
-      for (int r = 0; r < KEYS_EACH; ++r)
-#pragma unroll
-        for (int u = 0; u < T::PIECES; ++u) {
-          int at = (T::VEC * m + 16 * T::VEC * u) * T::E;
-          if (PAD) at = at < bytes ? at : 0;
-          held.v[b][r][u] = __builtin_nontemporal_load((const VWords *)(row + r * (hd * T::E) + at));
-        }
-    }
+      for (int u = 0; u < T::PIECES; ++u) {
+        int at = (T::VEC * m + 16 * T::VEC * u) * T::E;
+        if (PAD) at = at < bytes ? at : 0;
+        held.v[r][u] = __builtin_nontemporal_load((const VWords *)(row + r * (hd * T::E) + at));
+      }
   }
 
   // The queries as B operands: chunk u of quarter j is d = (4 u + j) PER .. + PER - 1, as K's.
@@ -206,18 +212,18 @@ struct Wave {
       for (int w = 0; w < T::PER / 4; ++w) raw.x[i][w] = query(rows, cols, first + i * step, w);
   }
   // float16 parts hold 22 bits of a number between two of them, down to 2^-24: the largest of a row is brought to 2^14 .. 2^15
-  __device__ __forceinline__ void find_down(const float *rows, int cols) {
+  __device__ __forceinline__ static float larger(float most, f32x4 x) {
+    return fmaxf(most, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))));
+  }
+  __device__ __forceinline__ float largest(const Raw &raw) const {  // of this wavefront's share
     float most = 0.0f;
 #pragma unroll
-    for (int u = 0; u < T::CHUNKS; ++u)
+    for (int i = 0; i < SHARE; ++i)
 #pragma unroll
-      for (int w = 0; w < T::PER / 4; ++w) {
-        const f32x4 x = query(rows, cols, u, w);
-        most = fmaxf(most, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))));
-      }
-    most = max_across_quarters(most);
-    down = most > 0.0f && most < INFINITY ? 15 - __builtin_amdgcn_frexp_expf(most) : 0;
+      for (int w = 0; w < T::PER / 4; ++w) most = larger(most, raw.x[i][w]);
+    return max_across_quarters(most);
   }
+  __device__ __forceinline__ void set_down(float most) { down = most > 0.0f && most < INFINITY ? 15 - __builtin_amdgcn_frexp_expf(most) : 0; }
   __device__ __forceinline__ void put_query(u32x4 *to, const f32x4 (&x)[T::PER / 4], int u) const {
     u32x4 part[T::PARTS];
     if constexpr (DTYPE == kPageF32) {
@@ -239,7 +245,15 @@ struct Wave {
       if (first + i * step < T::CHUNKS) put_query(to, raw.x[i], first + i * step);
   }
   // ... all of them by this wavefront, for itself
-  __device__ __forceinline__ void own_queries(u32x4 *to, const float *rows, int cols) const {
+  __device__ __forceinline__ void own_queries(u32x4 *to, const float *rows, int cols) {
+    if constexpr (DTYPE == kPageF16) {
+      float most = 0.0f;
+#pragma unroll
+      for (int u = 0; u < T::CHUNKS; ++u)
+#pragma unroll
+        for (int w = 0; w < T::PER / 4; ++w) most = larger(most, query(rows, cols, u, w));
+      set_down(max_across_quarters(most));
+    }
 #pragma unroll
     for (int u = 0; u < T::CHUNKS; ++u) {
       f32x4 x[T::PER / 4];
@@ -276,8 +290,7 @@ struct Wave {
   }
   __device__ __forceinline__ void ask(int first, int last) {
     // (the entries are waited for here, where nothing is behind them yet)
-#pragma unroll
-    for (int b = 0; b < T::BLOCKS; ++b) asm volatile("" : "+v"(now.k[b]), "+v"(now.v[b]), "+v"(next.k[b]), "+v"(next.v[b]));
+    asm volatile("" : "+v"(now.k), "+v"(now.v), "+v"(next.k), "+v"(next.v));
     if (first >= last) return;
     ask_k(now, first);
     ask_v(now, first);
@@ -288,28 +301,24 @@ struct Wave {
   // however the code is reached, and an address that came by a load behind others would wait for all of them.)
   template <bool MORE>
   __device__ __forceinline__ void take(int tile, int then, int after) {
-    f32x4 x[T::BLOCKS][T::S];
+    f32x4 x[T::S];
 #pragma unroll
-    for (int b = 0; b < T::BLOCKS; ++b)
-#pragma unroll
-      for (int s = 0; s < T::S; ++s) x[b][s] = f32x4{0, 0, 0, 0};
+    for (int s = 0; s < T::S; ++s) x[s] = f32x4{0, 0, 0, 0};
 #pragma unroll
     for (int part = T::PARTS - 1; part >= 0; --part)
 #pragma unroll
       for (int u = 0; u < T::CHUNKS; ++u) {
         const u32x4 mine = q[(part * T::CHUNKS + u) * 64 + lane];
 #pragma unroll
-        for (int b = 0; b < T::BLOCKS; ++b)
+        for (int s = 0; s < T::S; ++s) {
+          if constexpr (DTYPE == kPageF32) {
+            const f32x4 k = __builtin_bit_cast(f32x4, held.k[s][u]), y = __builtin_bit_cast(f32x4, mine);
 #pragma unroll
-          for (int s = 0; s < T::S; ++s) {
-            if constexpr (DTYPE == kPageF32) {
-              const f32x4 k = __builtin_bit_cast(f32x4, held.k[b][s][u]), y = __builtin_bit_cast(f32x4, mine);
-#pragma unroll
-              for (int e = 0; e < 4; ++e) x[b][s] = mfma_f32_16(k[e], y[e], x[b][s]);
-            } else {
-              x[b][s] = mfma16(held.k[b][s][u], mine, x[b][s]);
-            }
+            for (int e = 0; e < 4; ++e) x[s] = mfma_f32_16(k[e], y[e], x[s]);
+          } else {
+            x[s] = mfma16(held.k[s][u], mine, x[s]);
           }
+        }
       }
     const Pages its = next;
     if constexpr (MORE) {
@@ -317,30 +326,22 @@ struct Wave {
       ask_k(its, then);
     }
     // keys behind the sequence's end or in no page: no score, and a value that is no number would not vanish at weight 0
-    bool whole = true;
-#pragma unroll
-    for (int b = 0; b < T::BLOCKS; ++b) whole = whole && held.in[b];
     float most = -INFINITY;
-    if (__any(!whole || (tile + 1) * T::KEYS > len)) {
+    if (__any(!held.in || (tile + 1) * T::KEYS > len)) {
+      const int key = tile * T::KEYS + j * KEYS_EACH;
 #pragma unroll
-      for (int b = 0; b < T::BLOCKS; ++b) {
-        const int key = tile * T::KEYS + b * T::BLOCK_KEYS + j * KEYS_EACH;
+      for (int r = 0; r < KEYS_EACH; ++r)
+        if (!held.in || key + r >= len) {
+          x[r >> 2][r & 3] = -INFINITY;
 #pragma unroll
-        for (int r = 0; r < KEYS_EACH; ++r)
-          if (!held.in[b] || key + r >= len) {
-            x[b][r >> 2][r & 3] = -INFINITY;
-#pragma unroll
-            for (int u = 0; u < T::PIECES; ++u) held.v[b][r][u] = VWords{};
-          }
-      }
+          for (int u = 0; u < T::PIECES; ++u) held.v[r][u] = VWords{};
+        }
     }
 #pragma unroll
-    for (int b = 0; b < T::BLOCKS; ++b)
-#pragma unroll
-      for (int r = 0; r < KEYS_EACH; ++r) {
-        if constexpr (DTYPE == kPageF16) x[b][r >> 2][r & 3] = ldexpf(x[b][r >> 2][r & 3], -down);
-        most = fmaxf(most, x[b][r >> 2][r & 3]);
-      }
+    for (int r = 0; r < KEYS_EACH; ++r) {
+      if constexpr (DTYPE == kPageF16) x[r >> 2][r & 3] = ldexpf(x[r >> 2][r & 3], -down);
+      most = fmaxf(most, x[r >> 2][r & 3]);
+    }
     most = max_across_quarters(most) * c;
     if (__any(most > top)) {
       const float now = fmaxf(top, most);
@@ -354,42 +355,39 @@ struct Wave {
     }
     // (float16 parts of a weight: lifted by 2^15, as the queries are; the sum is lifted with them)
     const float from = top == -INFINITY ? 0.0f : DTYPE == kPageF16 ? top - 15.0f : top;
+    float w[KEYS_EACH];
 #pragma unroll
-    for (int b = 0; b < T::BLOCKS; ++b) {
-      float w[KEYS_EACH];
+    for (int r = 0; r < KEYS_EACH; ++r) {
+      w[r] = __builtin_amdgcn_exp2f(fmaf(x[r >> 2][r & 3], c, -from));
+      sum += w[r];
+    }
+    if constexpr (DTYPE == kPageF32) {
 #pragma unroll
-      for (int r = 0; r < KEYS_EACH; ++r) {
-        w[r] = __builtin_amdgcn_exp2f(fmaf(x[b][r >> 2][r & 3], c, -from));
-        sum += w[r];
-      }
-      if constexpr (DTYPE == kPageF32) {
+      for (int r = 0; r < KEYS_EACH; ++r)
 #pragma unroll
-        for (int r = 0; r < KEYS_EACH; ++r)
+        for (int u = 0; u < T::PIECES; ++u) {
+          typedef float Columns __attribute__((ext_vector_type(T::WORDS)));
+          const Columns columns = __builtin_bit_cast(Columns, held.v[r][u]);
 #pragma unroll
-          for (int u = 0; u < T::PIECES; ++u) {
-            typedef float Columns __attribute__((ext_vector_type(T::WORDS)));
-            const Columns columns = __builtin_bit_cast(Columns, held.v[b][r][u]);
+          for (int e = 0; e < T::VEC; ++e) acc[u][e] = mfma_f32_16(columns[e], w[r], acc[u][e]);
+        }
+    } else {
+      u32x4 weights[T::PARTS];
+      if constexpr (DTYPE == kPageBf16)
+        split_octet(f32x4{w[0], w[1], w[2], w[3]}, f32x4{w[4], w[5], w[6], w[7]}, weights[0], weights[1], weights[2]);
+      else
+        split_f16(w, weights[0], weights[1]);
 #pragma unroll
-            for (int e = 0; e < T::VEC; ++e) acc[u][e] = mfma_f32_16(columns[e], w[r], acc[u][e]);
-          }
-      } else {
-        u32x4 weights[T::PARTS];
-        if constexpr (DTYPE == kPageBf16)
-          split_octet(f32x4{w[0], w[1], w[2], w[3]}, f32x4{w[4], w[5], w[6], w[7]}, weights[0], weights[1], weights[2]);
-        else
-          split_f16(w, weights[0], weights[1]);
+      for (int u = 0; u < T::PIECES; ++u)
 #pragma unroll
-        for (int u = 0; u < T::PIECES; ++u)
+        for (int e = 0; e < T::VEC; ++e) {
+          u32x4 column;
 #pragma unroll
-          for (int e = 0; e < T::VEC; ++e) {
-            u32x4 column;
+          for (int r = 0; r < 4; ++r)
+            column[r] = __builtin_amdgcn_perm(held.v[2 * r + 1][u][e >> 1], held.v[2 * r][u][e >> 1], e & 1 ? 0x07060302u : 0x05040100u);
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-              column[r] = __builtin_amdgcn_perm(held.v[b][2 * r + 1][u][e >> 1], held.v[b][2 * r][u][e >> 1], e & 1 ? 0x07060302u : 0x05040100u);
-#pragma unroll
-            for (int part = T::PARTS - 1; part >= 0; --part) acc[u][e] = mfma16(column, weights[part], acc[u][e]);
-          }
-      }
+          for (int part = T::PARTS - 1; part >= 0; --part) acc[u][e] = mfma16(column, weights[part], acc[u][e]);
+        }
     }
     if constexpr (MORE) ask_v(its, then);
   }
@@ -429,7 +427,7 @@ __global__ __launch_bounds__((64 * Tile<DTYPE, HD>::WAVES), (Tile<DTYPE, HD>::WA
   constexpr int QUERIES = T::PARTS * T::CHUNKS * 64 * 4, OUTS = WAVES * kCols * STRIDE;
   __shared__ __align__(16) float shared[QUERIES + (OUTS > (WAVES - 1) * QUERIES ? OUTS : (WAVES - 1) * QUERIES)];
   auto outs = [&](int v, int n, int d) { return shared + QUERIES + (v * kCols + n) * STRIDE + d; };
-  __shared__ float tops[WAVES][kCols], sums[WAVES][kCols];
+  __shared__ float tops[WAVES][kCols], sums[WAVES][kCols], larges[WAVES][kCols];
   __shared__ int scan[WAVES], held[WAVES], longest[WAVES], last_one;
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
   // (values from LDS that are the same in all lanes are said to be: they live in scalar registers then)
@@ -494,10 +492,11 @@ __global__ __launch_bounds__((64 * Tile<DTYPE, HD>::WAVES), (Tile<DTYPE, HD>::WA
       for (int i = t; i < a.H * hd; i += THREADS) a.out[r * a.out_stride + i] = 0.0f;
   const long long total = (long long)row_tiles * pairs, n_pairs = (long long)some * pairs;
   int mode = kSpans;
-  long long unit = max(1LL, (total + wgs - 1) / wgs);  // tiles of a span, or of a chunk at most
+  const long long share = (total + wgs - 1) / wgs;
+  long long unit = max(1LL, (total + kBegin * n_pairs + wgs - 1) / wgs);  // of a span; or tiles of a chunk, at most
   if (n_pairs > wgs && most <= kWavefrontTiles) {
     mode = kWavefronts;
-  } else if (unit < kShortSpan && n_pairs <= wgs) {
+  } else if (share < kShortSpan && n_pairs <= wgs) {
     // chunks of pairs, one a workgroup: sum of ceil(tiles / unit) <= total / unit + pairs
     mode = kChunks;
     unit = n_pairs < wgs && most > T::WHOLE ? max((long long)quotient(total + (wgs - n_pairs) - 1, wgs - n_pairs), (long long)WAVES) : most;
@@ -505,7 +504,7 @@ __global__ __launch_bounds__((64 * Tile<DTYPE, HD>::WAVES), (Tile<DTYPE, HD>::WA
   if (mode != kWavefronts) {  // units of one kv head before each row
     auto units_of = [&](int r) {
       const int tiles = tiles_of(known_length(r));
-      return mode == kSpans ? tiles : quotient(tiles + unit - 1, unit);
+      return mode == kSpans ? (tiles > 0 ? tiles + kBegin : 0) : quotient(tiles + unit - 1, unit);
     };
     if (few) {
       const int mine = lane < a.rows ? units_of(lane) : 0, upto = sum_lanes(mine);
@@ -584,13 +583,15 @@ __global__ __launch_bounds__((64 * Tile<DTYPE, HD>::WAVES), (Tile<DTYPE, HD>::WA
       const long long begins = of_row + (long long)s.pair * units;
       const int from = (int)(at - begins);
       if (mode == kSpans) {
-        s.first = from;
-        s.last = (int)(min(end, begins + units) - begins);
-        at += s.last - s.first;
-        s.first_wg = quotient(begins, unit);
+        const long long first_tile = begins + kBegin;
+        s.first = max(from - kBegin, 0);
+        s.last = (int)(min(end, begins + units) - first_tile);
+        at = min(end, begins + units);
+        if (s.last <= s.first) continue;
+        s.first_wg = quotient(first_tile, unit);
         s.last_wg = quotient(begins + units - 1, unit);
-        s.late = begins > blockIdx.x * unit;
-        s.first_late = begins > s.first_wg * unit;
+        s.late = first_tile > blockIdx.x * unit;
+        s.first_late = first_tile > s.first_wg * unit;
       } else {  // equal shares
         s.first = quotient((long long)tiles * from, units);
         s.last = quotient((long long)tiles * (from + 1), units);
@@ -605,8 +606,8 @@ __global__ __launch_bounds__((64 * Tile<DTYPE, HD>::WAVES), (Tile<DTYPE, HD>::WA
   };
 
   // Of two workgroups on a compute unit the first one's requests go before the other's: with equal spans the first ones ended at
-  // 77 to 100 us and the others at 108 to 118 (16 sequences of 2048 to 8192 keys, float32).  The others' instructions go
-  // first, therefore: half to one per cent of most launches.  (Spans of unequal lengths, or short ones for whoever is
+  // 77 to 100 us and the others at 108 to 118 (16 sequences of 2048 to 8192 keys, float32, two on each).  The others' instructions
+  // go first, therefore: half to one per cent of most launches.  (Spans of unequal lengths, or short ones for whoever is
   // ready, cost more in parts of pairs than they gave: 110 -> 113 and 121 us.)
   if (PER_CU == 2 && (int)blockIdx.x >= wgs / 2) __builtin_amdgcn_s_setprio(3);
   Wave<DTYPE, HD, PAD> w(p, a.scale);
@@ -625,17 +626,33 @@ __global__ __launch_bounds__((64 * Tile<DTYPE, HD>::WAVES), (Tile<DTYPE, HD>::WA
     if (!alone) w.ask_queries(raw, rows_of(s), cols_of(s), wave, WAVES);
     w.ask(s.first + mine, s.last);
   };
+  auto put_largest = [&] {  // (before a barrier, and put_queries behind it)
+    if constexpr (DTYPE == kPageF16) {
+      const float most = w.largest(raw);
+      if (lane < kCols) larges[wave][lane] = most;
+    }
+  };
   auto put_queries = [&](const Segment &s) {
-    if constexpr (DTYPE == kPageF16) w.find_down(rows_of(s), cols_of(s));
-    if (alone)
+    if (alone) {
       w.own_queries(queries, rows_of(s), cols_of(s));
-    else
-      w.put_queries(queries, raw, wave, WAVES);
+      return;
+    }
+    if constexpr (DTYPE == kPageF16) {
+      float most = larges[0][w.m];
+#pragma unroll
+      for (int v = 1; v < WAVES; ++v) most = fmaxf(most, larges[v][w.m]);
+      w.set_down(most);
+    }
+    w.put_queries(queries, raw, wave, WAVES);
   };
   Segment s;
   bool more = next_segment(s);
   if (more) {
     start(s);
+    if (DTYPE == kPageF16 && !alone) {  // (then all wavefronts have the same segment)
+      put_largest();
+      __syncthreads();
+    }
     put_queries(s);
   }
   __syncthreads();
@@ -682,6 +699,7 @@ __global__ __launch_bounds__((64 * Tile<DTYPE, HD>::WAVES), (Tile<DTYPE, HD>::WA
 #pragma unroll
           for (int e = 0; e < T::VEC; ++e)
             *outs(wave, w.m, T::VEC * (4 * w.j + i) + 16 * T::VEC * u + e) = w.acc[u][e][i] * fade;
+    if (more) put_largest();
     __syncthreads();
     if (more) put_queries(s);  // (nobody reads the old ones any more)
     const bool whole = now.first_wg == now.last_wg;
@@ -856,9 +874,10 @@ hipError_t launch_attend(const PagedAttendArgs &a, const PagePool &p, hipStream_
   return hipGetLastError();
 }
 // One workgroup on a compute unit reads long stretches of few pairs faster than two, of which the first gets ahead: 16 sequences of 2048 to
-// 8192 keys (128 pairs, float32) 106 us | two 109, one of 131072 (4 pairs, bfloat16) 50 | 53, 24 of 20 to 700 (192 pairs) 10.2 | 11.9.
-// Where there are more pairs than compute units two hide each other's beginnings and ends: 64 sequences of 100 to
-// 300 keys (512 pairs) 29 | 15 us, 77 of up to 5000 (308 pairs) 81 | 72.
+// 8192 keys (128 pairs, float32) 105.5 us | two 106.7, one of 131072 (4 pairs, bfloat16) 50 | 53, 24 of 20 to 700 (192 pairs) 10.9 | 12.1.
+// Where there are more pairs than compute units two hide each other's beginnings and ends: 64 sequences of 100 to 300 keys
+// (512 pairs, float32) two 25 us | one 33, 39 of up to 5000 (312 pairs of heads of 64) 38 | 46.  (512 long pairs would like one: 64 of 8192
+// to 32768 keys 766 us | 781; how long they are is known on the device only.)
 template <int DTYPE, int HD>
 hipError_t launch_attend(const PagedAttendArgs &a, const PagePool &p, hipStream_t stream) {
   if constexpr (HD == 256) {  // (registers for one)

@@ -101,6 +101,14 @@ int check_pair(const shainet_attn_ctx *c, const shainet_paged_cache *pc, int lay
   return check_device(pc);
 }
 
+// Calls whose work depends on what the host knows now, or that wait: good for one execution only.
+int refuse_recording(const shainet_attn_ctx *c, const char *what) {
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  if (c->stream) HIP_TRY(hipStreamIsCapturing(c->stream, &status));
+  if (status == hipStreamCaptureStatusNone) return SHAINET_HIP_OK;
+  return fail(SHAINET_HIP_ERR_ARGUMENT, "%s cannot be recorded", what);
+}
+
 int refuse_unknown_lengths(const shainet_paged_cache *pc, const char *what) {
   if (!pc->lengths_on_device) return SHAINET_HIP_OK;
   return fail(SHAINET_HIP_ERR_ARGUMENT, "%s: the lengths were changed on the device; call shainet_paged_cache_lengths_from_device first", what);
@@ -128,13 +136,14 @@ MapArgs map_of(const shainet_paged_cache *pc) {
   return a;
 }
 
-// The lengths of up to kMaxSeqs sequences that the host knows change by `change`; rows (nullable): three lists of max_rows.
-int map_listed(shainet_paged_cache *pc, const int *ids, const int *change, int n, int *rows, int max_rows) {
+// The lengths of up to kMaxSeqs sequences, `was` as far as the host knows, change by `change`; rows (nullable): three lists of max_rows.
+int map_listed(shainet_paged_cache *pc, const int *ids, const int *was, const int *change, int n, int *rows, int max_rows) {
   MapArgs a = map_of(pc);
   a.n = n;
   a.inlined = 1;
   for (int i = 0; i < n; ++i) {
     a.id[i] = ids[i];
+    a.was[i] = was[i];
     a.change[i] = change[i];
   }
   a.max_rows = max_rows;
@@ -147,15 +156,18 @@ int map_listed(shainet_paged_cache *pc, const int *ids, const int *change, int n
   return e == hipSuccess ? SHAINET_HIP_OK : hip_fail(e, "map launch");
 }
 
-// The cos/sin table reaches as far as a sequence can: which positions a map holds is known to the device only.
-int reach_table(shainet_attn_ctx *c, const shainet_paged_cache *pc) {
-  if (c->rope_positions >= reach_of(pc)) return SHAINET_HIP_OK;
-  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-  if (c->stream) HIP_TRY(hipStreamIsCapturing(c->stream, &status));
-  if (status != hipStreamCaptureStatusNone)
+// Positions that a map of rows can give; a caller's own lists may name any that the table holds.
+long long mapped_reach(const shainet_paged_cache *pc) { return (long long)(pc->seq_pages < pc->n_pages ? pc->seq_pages : pc->n_pages) << pc->shift; }
+
+// The cos/sin table goes as far as rows can: at which positions they are is known to the device only.
+int reach_table(shainet_attn_ctx *c, long long reach) {
+  if (c->rope_positions >= reach) return SHAINET_HIP_OK;
+  if (refuse_recording(c, ""))
     return fail(SHAINET_HIP_ERR_ARGUMENT, "the context's cos/sin table must be extended to %lld positions, which cannot be recorded: create the context "
-                "with that many, or place rows once before recording", reach_of(pc));
-  return ensure_rope_table(c, (int)reach_of(pc));
+                "with that many, or place rows once before recording", reach);
+  if (reach * c->hd * 4 > 8LL << 30)
+    return fail(SHAINET_HIP_ERR_ALLOC, "a cos/sin table of %lld positions would take more than 8 GiB: the cache's table is that wide", reach);
+  return ensure_rope_table(c, (int)reach);
 }
 
 PrepArgs prep_of(const shainet_attn_ctx *c, const float *q, long long q_stride, const float *k, long long k_stride, const float *v,
@@ -230,6 +242,7 @@ int shainet_paged_cache_create(shainet_paged_cache **out, shainet_attn_ctx *ctx,
   if (layers < 1 || n_pages < 1 || seq_pages < 1 || (long long)n_pages * page_rows > 0x7fffffffLL ||
       (long long)seq_pages * page_rows > 0x3fffffffLL || (long long)n_seqs * seq_pages > 0x7fffffffLL)
     return fail(SHAINET_HIP_ERR_ARGUMENT, "invalid cache geometry: slots and table entries are 32-bit numbers, positions 30-bit ones");
+  if (int rc = refuse_recording(ctx, "shainet_paged_cache_create")) return rc;
   shainet_paged_cache *pc = new (std::nothrow) shainet_paged_cache();
   if (!pc) return fail(SHAINET_HIP_ERR_ALLOC, "out of host memory");
   pc->ctx = ctx;
@@ -331,6 +344,7 @@ int shainet_paged_cache_map_rows(shainet_paged_cache *pc, const int *seq_ids, co
 int shainet_paged_cache_lengths_from_device(shainet_paged_cache *pc) {
   if (!pc) return fail(SHAINET_HIP_ERR_ARGUMENT, "cache is null");
   if (int rc = check_device(pc)) return rc;
+  if (int rc = refuse_recording(pc->ctx, "shainet_paged_cache_lengths_from_device")) return rc;
   HIP_TRY(hipMemcpyAsync(pc->pin, pc->lens, pc->n_seqs * sizeof(int), hipMemcpyDeviceToHost, pc->ctx->stream));
   HIP_TRY(hipMemcpyAsync(pc->pin + pc->n_seqs, pc->n_free, sizeof(int), hipMemcpyDeviceToHost, pc->ctx->stream));
   HIP_TRY(hipStreamSynchronize(pc->ctx->stream));
@@ -360,9 +374,10 @@ int shainet_paged_cache_truncate(shainet_paged_cache *pc, int seq, int len) {
   if (int rc = refuse_unknown_lengths(pc, "shainet_paged_cache_truncate")) return rc;
   if (len < 0 || len > pc->len[seq]) return fail(SHAINET_HIP_ERR_ARGUMENT, "truncate to %d outside 0..%d", len, pc->len[seq]);
   if (int rc = check_device(pc)) return rc;
-  const int change = len - pc->len[seq];
+  if (int rc = refuse_recording(pc->ctx, "shainet_paged_cache_truncate")) return rc;
+  const int was = pc->len[seq], change = len - was;
   if (change == 0) return SHAINET_HIP_OK;
-  if (int rc = map_listed(pc, &seq, &change, 1, nullptr, 0)) return rc;
+  if (int rc = map_listed(pc, &seq, &was, &change, 1, nullptr, 0)) return rc;
   pc->free_count += pages_of(pc, pc->len[seq]) - pages_of(pc, len);
   pc->len[seq] = len;
   forget_rows(pc);
@@ -373,6 +388,7 @@ int shainet_paged_cache_clear(shainet_paged_cache *pc, int seq) {
   if (!pc || seq >= pc->n_seqs) return fail(SHAINET_HIP_ERR_ARGUMENT, "invalid sequence");
   if (seq >= 0) return shainet_paged_cache_truncate(pc, seq, 0);
   if (int rc = check_device(pc)) return rc;
+  if (int rc = refuse_recording(pc->ctx, "shainet_paged_cache_clear")) return rc;
   const hipError_t e = launch_page_reset(pc->lens, pc->n_seqs, pc->free_pages, pc->n_free, pc->n_pages, pc->ctx->stream);
   if (e != hipSuccess) return hip_fail(e, "reset launch");
   pc->len.assign(pc->n_seqs, 0);
@@ -389,6 +405,7 @@ int shainet_paged_cache_read(shainet_paged_cache *pc, int layer, int seq, int kv
   if ((long long)pos0 + n > pc->len[seq]) return fail(SHAINET_HIP_ERR_ARGUMENT, "rows %d..%lld of a sequence of %d", pos0, (long long)pos0 + n - 1, pc->len[seq]);
   if (n == 0) return SHAINET_HIP_OK;
   if (int rc = check_device(pc)) return rc;
+  if (int rc = refuse_recording(pc->ctx, "shainet_paged_cache_read")) return rc;
   const size_t each = (size_t)pc->KV * n * pc->hd;
   if (int rc = pc->gathered.reserve(2 * each)) return rc;
   float *k = pc->gathered.p, *v = k + each;
@@ -409,7 +426,7 @@ int shainet_attn_append_paged(shainet_attn_ctx *c, shainet_paged_cache *pc, int 
   if (rows < 1 || rows > 0x3fffffff / (c->H + 2 * c->KV)) return fail(SHAINET_HIP_ERR_ARGUMENT, "rows must be in 1..%d", 0x3fffffff / (c->H + 2 * c->KV));
   if (q_stride < (long long)c->H * c->hd || k_stride < (long long)c->KV * c->hd || v_stride < (long long)c->KV * c->hd)
     return fail(SHAINET_HIP_ERR_ARGUMENT, "row strides must be at least the row widths %d and %d", c->H * c->hd, c->KV * c->hd);
-  if (int rc = reach_table(c, pc)) return rc;
+  if (int rc = reach_table(c, reach_of(pc))) return rc;
   return append(c, pc, layer, prep_of(c, q, q_stride, k, k_stride, v, v_stride, q_rot), slots, positions, rows);
 }
 
@@ -431,7 +448,7 @@ int shainet_attn_step_paged(shainet_attn_ctx *c, shainet_paged_cache *pc, int la
   if (n < 1 || n > pc->n_seqs) return fail(SHAINET_HIP_ERR_ARGUMENT, "n must be in 1..%d", pc->n_seqs);
   if (layer > 0 && n != pc->step_rows)
     return fail(SHAINET_HIP_ERR_ARGUMENT, "layer %d of a step of %d rows: layer 0 mapped %d", layer, n, pc->step_rows);
-  if (int rc = reach_table(c, pc)) return rc;
+  if (int rc = reach_table(c, mapped_reach(pc))) return rc;
   if (layer == 0) {
     MapArgs a = map_of(pc);
     a.n = n;
@@ -459,6 +476,7 @@ int shainet_attn_forward_paged(shainet_attn_ctx *c, shainet_paged_cache *pc, int
   if (mem != SHAINET_HIP_MEM_HOST && mem != SHAINET_HIP_MEM_DEVICE)
     return fail(SHAINET_HIP_ERR_ARGUMENT, "mem must be SHAINET_HIP_MEM_HOST or SHAINET_HIP_MEM_DEVICE");
   if (n_seqs < 1 || n_seqs > SHAINET_HIP_MAX_BATCH) return fail(SHAINET_HIP_ERR_ARGUMENT, "n_seqs must be in 1..%d", SHAINET_HIP_MAX_BATCH);
+  if (int rc = refuse_recording(c, "shainet_attn_forward_paged")) return rc;
   if (int rc = refuse_unknown_lengths(pc, "shainet_attn_forward_paged")) return rc;
   int ids[kMaxSeqs], start[kMaxSeqs], change[kMaxSeqs], longest = 0;
   long long total = 0, pages = 0;
@@ -484,7 +502,7 @@ int shainet_attn_forward_paged(shainet_attn_ctx *c, shainet_paged_cache *pc, int
     return fail(SHAINET_HIP_ERR_ARGUMENT, "layer %d: other rows than layer 0 of this cache had last", layer);
   const int rows = (int)total;
   const size_t q_floats = (size_t)rows * c->H * c->hd, kv_floats = (size_t)rows * c->KV * c->hd, gathered = (size_t)c->KV * longest * c->hd;
-  int rc = reach_table(c, pc);
+  int rc = reach_table(c, mapped_reach(pc));
   if (!rc) rc = c->q_rot.reserve(q_floats);
   if (!rc && layer == 0) rc = pc->rows.reserve(3 * (size_t)rows);
   if (!rc && longest) rc = pc->gathered.reserve(2 * gathered);
@@ -521,7 +539,7 @@ int shainet_attn_forward_paged(shainet_attn_ctx *c, shainet_paged_cache *pc, int
       pc->last_ids.clear();
       rc = fail(SHAINET_HIP_ERR_ALLOC, "out of host memory");
     }
-    if (!rc) rc = map_listed(pc, ids, change, n_seqs, lists, rows);
+    if (!rc) rc = map_listed(pc, ids, start, change, n_seqs, lists, rows);
     if (rc) {
       if (mem == SHAINET_HIP_MEM_HOST) (void)hipStreamSynchronize(c->stream);
       return rc;
@@ -551,8 +569,11 @@ int shainet_attn_forward_paged(shainet_attn_ctx *c, shainet_paged_cache *pc, int
   }
   if (rc) {
     if (layer == 0) {  // the rows leave again: the call did not happen
-      for (int s = 0; s < n_seqs; ++s) change[s] = -change[s];
-      (void)map_listed(pc, ids, change, n_seqs, nullptr, 0);
+      for (int s = 0; s < n_seqs; ++s) {
+        start[s] += change[s];
+        change[s] = -change[s];
+      }
+      (void)map_listed(pc, ids, start, change, n_seqs, nullptr, 0);
       pc->last_ids.clear();
     }
     if (mem == SHAINET_HIP_MEM_HOST) (void)hipStreamSynchronize(c->stream);
@@ -570,6 +591,7 @@ int shainet_attn_forward_paged(shainet_attn_ctx *c, shainet_paged_cache *pc, int
     if (ce != hipSuccess) return hip_fail(ce, "hipMemcpyAsync(out)");
     if (se != hipSuccess) return hip_fail(se, "hipStreamSynchronize");
     memcpy(out, c->pin_out.p, q_floats * sizeof(float));
+    if (int of_map = check_error_word(pc->ctx->error)) return of_map;
     return check_error_word(c->error);
   }
   return SHAINET_HIP_OK;

@@ -134,7 +134,7 @@ __global__ __launch_bounds__(THREADS) void page_map_kernel(MapArgs a) {
     if (atomicOr(&named[s >> 5], 1u << (s & 31)) >> (s & 31) & 1) wrong = true;
     const int len = a.lens[s];
     const long long now = (long long)len + d;
-    if (len < 0 || len > most || now < 0) {
+    if (len < 0 || len > most || now < 0 || (a.inlined && len != a.was[t * each + u])) {
       wrong = true;
       continue;
     }
@@ -238,13 +238,17 @@ hipError_t launch_page_map(const MapArgs &a, hipStream_t stream) {
   if (a.n < 1 || a.n > kMaxPagedSeqs || a.n_seqs > kMaxPagedSeqs || (a.inlined && a.n > kMaxSeqs) || a.max_rows < 0 ||
       (a.max_rows && (!a.slots || !a.positions || !a.row_seqs)))
     return hipErrorInvalidValue;
-  // What a decode step moves is done by a few wavefronts, whose barriers take less; more rows, or pages by the thousand, by a
-  // workgroup, and by one on each compute unit.
-  if (a.n <= 256 && a.max_rows <= 1024 && a.n_pages <= 1 << 16) {
+  // A decode step's rows are mapped by one workgroup of four wavefronts, whose barriers take less: 16 sequences and their inverse 8.9 us a
+  // pair of calls where the pool has 60000 pages | 10.9 us by 1024 threads on each of up to 256 compute units (15.4 where it has a
+  // million).  Pages by the ten thousand, which an entry may give back, want those: 8192 in one call 10.6 us | 3.0, 32768 37 | 4.
+  // (The many are as fast as one of them where two would do: 1500 rows of 300 sequences 5.3 us | 5.6, 8000 5.3 | 10.9.)
+  const long long of_entries = a.delta || a.inlined ? (long long)a.n * a.seq_pages : a.n;  // pages that can move, at most
+  const int pages = (int)(of_entries < a.n_pages ? of_entries : a.n_pages);
+  if (a.n <= 256 && a.max_rows <= 1024 && pages <= 1 << 16) {
     hipLaunchKernelGGL(page_map_kernel<256>, dim3(1), dim3(256), 0, stream, a);
   } else {
-    const int items = a.max_rows > a.n_pages ? a.max_rows : a.n_pages, blocks = (items + 1023) / 1024;
-    hipLaunchKernelGGL(page_map_kernel<1024>, dim3((unsigned)(blocks <= 4 ? 1 : blocks < 256 ? blocks : 256)), dim3(1024), 0, stream, a);
+    const int items = a.max_rows > pages ? a.max_rows : pages, blocks = (items + 1023) / 1024;
+    hipLaunchKernelGGL(page_map_kernel<1024>, dim3((unsigned)(blocks < 1 ? 1 : blocks < 256 ? blocks : 256)), dim3(1024), 0, stream, a);
   }
   return hipGetLastError();
 }

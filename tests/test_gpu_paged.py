@@ -775,3 +775,147 @@ def test_steps_on_another_stream(hip, torch):
     cache.lengths_from_device()
     assert [cache.len(s) for s in range(3)] == [6, 6, 6]
     ctx.set_stream(torch.cuda.current_stream().cuda_stream)
+
+
+# ---- recordings, and what the host knows ------------------------------------------------------------
+
+def _rows(torch, rng, n, H, KV, hd):
+    return [torch.from_numpy(rng.standard_normal((n, w * hd)).astype(np.float32)).cuda() for w in (H, KV, KV)]
+
+
+def test_a_recorded_step_outlives_the_table_of_angles(hip, torch):
+    """A longer table of angles, made for another cache, leaves recordings the one that they read."""
+    H, KV, hd = 4, 2, 64
+    rng = np.random.default_rng(11)
+    stream = torch.cuda.Stream()
+    ctx = hip.AttnContext(H, KV, hd, max_positions=64)
+    ctx.set_stream(stream.cuda_stream)
+    caches = [hip.PagedKVCache(ctx, 16, 8, 2, 8, dtype="f32") for _ in range(2)]
+    x = _rows(torch, rng, 2, H, KV, hd)
+    outs = [torch.zeros_like(x[0]) for _ in caches]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        ctx.step_paged(caches[0], *x, outs[0])
+    for turn in range(4):
+        if turn == 2:
+            longer = hip.PagedKVCache(ctx, 64, 64, 1, 64)
+            ctx.step_paged(longer, *(t[:1].contiguous() for t in x), torch.empty_like(x[0][:1]))
+            ctx.sync()
+            waste = [torch.full((64 * 32 * 2,), float("nan"), device="cuda") for _ in range(64)]
+        for t in x:
+            t.copy_(torch.from_numpy(rng.standard_normal(t.shape).astype(np.float32)))
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            graph.replay()
+        ctx.step_paged(caches[1], *x, outs[1])
+        ctx.sync()
+        assert torch.equal(*outs), turn
+    del waste
+
+
+def test_a_table_wider_than_the_pool(hip, torch):
+    """Sequences may be as wide as 2^30 rows where the pool holds a few thousand: angles are made for those."""
+    H, KV, hd = 4, 2, 64
+    rng = np.random.default_rng(12)
+    ctx = _ctx(hip, torch, H, KV, hd)
+    cache, plain = hip.PagedKVCache(ctx, 4, 1024, 1, 2 ** 20 - 1, dtype="f32"), hip.KVCache(ctx, 1, 4096)
+    for n in (1500, 1, 3, 2000, 1):
+        x = _rows(torch, rng, n, H, KV, hd)
+        got, want = ctx.forward_paged(cache, *x, [n]), ctx.forward(plain, *x, [n])
+        assert (got - want).abs().max().item() <= 2e-5, n
+    with pytest.raises(hip.HipError, match="pages wanted"):
+        ctx.forward_paged(cache, *_rows(torch, rng, 592, H, KV, hd), [592])
+    x = _rows(torch, rng, 1, H, KV, hd)
+    got = ctx.step_paged(cache, *x, torch.empty_like(x[0]))
+    assert (got - ctx.forward(plain, *x, [1])).abs().max().item() <= 2e-5
+    ctx.sync()
+    one = _ints(torch, [0])
+    with pytest.raises(hip.HipError, match="GiB"):  # of lists of the caller's own nothing is known
+        ctx.append_paged(cache, one, one, *x, torch.empty_like(x[0]))
+
+
+def test_calls_that_are_not_recorded(hip, torch):
+    H, KV, hd = 4, 2, 64
+    rng = np.random.default_rng(13)
+    stream = torch.cuda.Stream()
+    ctx = hip.AttnContext(H, KV, hd)
+    ctx.set_stream(stream.cuda_stream)
+    cache = hip.PagedKVCache(ctx, 16, 8, 2, 8)
+    x = _rows(torch, rng, 12, H, KV, hd)
+    ctx.forward_paged(cache, *x, [9, 3])
+    out = torch.zeros_like(x[0])
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=stream):
+        torch.add(out, 1, out=out)
+        for call in (lambda: cache.truncate(0, 3), lambda: cache.truncate(0, 9), lambda: cache.clear(), lambda: cache.clear(1),
+                     lambda: cache.read(0, 0, 0, 3), cache.lengths_from_device, lambda: hip.PagedKVCache(ctx, 16, 8, 2, 8),
+                     lambda: ctx.forward_paged(cache, *x, [9, 3])):
+            with pytest.raises(hip.ArgumentError, match="recorded"):
+                call()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert (out == 1).all() and cache.len(0) == 9 and cache.lens.tolist() == [9, 3] and cache.free_page_count() == 13
+    cache.truncate(0, 3)
+    assert cache.len(0) == 3
+    ctx.sync()
+    assert cache.lens.tolist() == [3, 3]
+
+
+@pytest.mark.parametrize("new", [[1, 2], [20, 1]])
+def test_lengths_that_the_host_missed(hip, torch, new):
+    """Replays that the host does not see: what it plans on its own lengths changes nothing and is reported."""
+    H, KV, hd = 4, 2, 64
+    rng = np.random.default_rng(14)
+    stream = torch.cuda.Stream()
+    ctx = hip.AttnContext(H, KV, hd)
+    ctx.set_stream(stream.cuda_stream)
+    cache, plain = hip.PagedKVCache(ctx, 32, 8, 2, 16, dtype="f32"), hip.KVCache(ctx, 2, 128)
+    x, more = _rows(torch, rng, 2, H, KV, hd), _rows(torch, rng, sum(new), H, KV, hd)
+    out = torch.zeros_like(x[0])
+    ctx.step_paged(cache, *x, out)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        ctx.step_paged(cache, *x, out)
+    cache.lengths_from_device()
+    for turn in range(3):
+        with torch.cuda.stream(stream):
+            graph.replay()
+        ctx.forward(plain, *x, [1, 1])
+    ctx.forward(plain, *x, [1, 1])
+    ctx.sync()
+    assert cache.len(0) == 1 and cache.lens.tolist() == [4, 4]
+    before = [t.clone() for t in (cache.table, cache.free_pages, cache.n_free, cache.k, cache.v)]
+    for call in (lambda: cache.truncate(1, 0), lambda: ctx.forward_paged(cache, *more, new)):
+        call()
+        with pytest.raises(hip.ArgumentError, match="did not know"):
+            ctx.sync()
+        assert cache.lens.tolist() == [4, 4]
+        for a, b in zip(before, (cache.table, cache.free_pages, cache.n_free, cache.k, cache.v)):
+            assert torch.equal(a, b)
+    cache.lengths_from_device()
+    assert [cache.len(s) for s in range(2)] == [4, 4]
+    got, want = ctx.forward_paged(cache, *more, new), ctx.forward(plain, *more, new)
+    ctx.sync()
+    assert (got - want).abs().max().item() <= 2e-5
+
+
+@pytest.mark.parametrize("seq_pages", [20000, 40000])
+def test_maps_of_many_pages(hip, torch, seq_pages):
+    """Pages by the ten thousand, in one workgroup and in many; a step of a large pool."""
+    n_pages, P = 70000, 8
+    cache, model = hip.PagedKVCache(_ctx(hip, torch, 1, 1, 8), n_pages, P, 3, seq_pages), Pages(n_pages, P, 3, seq_pages)
+    lists = [torch.empty(400000, dtype=torch.int32, device="cuda") for _ in range(3)]
+    few = [torch.empty(3, dtype=torch.int32, device="cuda") for _ in range(3)]
+    for entries, rows in (([(2, 150001), (0, 80003), (1, 160000)], lists), ([(1, -159999), (2, -1), (0, 3)], few), ([(0, -80006)], None),
+                          ([(2, 1), (1, -1), (0, 1)], few), ([(2, -150001), (0, -1)], None), ([(0, 160000)], lists)):
+        want = model.map(entries, rows[0].numel() if rows else 0)
+        cache.map_rows(_ints(torch, [d for _, d in entries]), *(rows or ()), seq_ids=_ints(torch, [s for s, _ in entries]))
+        cache.lengths_from_device()
+        _same_state(cache, model, len(model.free))
+        if rows:
+            got = np.stack([t[:len(want)].cpu().numpy() for t in rows], 1)
+            assert np.array_equal(got, np.array(want).reshape(-1, 3))
+            assert all((t[len(want):] == -1).all() for t in rows)
