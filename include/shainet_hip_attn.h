@@ -278,8 +278,8 @@ int shainet_attn_append_paged(shainet_attn_ctx *ctx, shainet_paged_cache *cache,
  * sequence row_seqs[r], by the table (the lengths are not looked at; several rows may name one sequence).  A row with
  * row_seqs outside 0..n_seqs-1 leaves its output alone; one with positions < 0, or whose keys' pages are all outside the
  * pool, gets zeros; one that sees an infinite number or none gets outputs that are infinite or no numbers.  At most
- * SHAINET_HIP_MAX_PAGED_SEQS rows, and rows * seq_pages * page_rows below 2^34.  Rows of q_rot and out at the given strides; out
- * may be q_rot.  Asynchronous on the context's stream.  Scores, softmax and sums are float32, keys and values the pages'
+ * SHAINET_HIP_MAX_PAGED_SEQS rows, and rows * seq_pages * page_rows below 2^34, times num_kv_heads (once for every 16 query
+ * heads of each) below 2^42.  Rows of q_rot and out at the given strides; out may be q_rot.  Asynchronous on the context's stream.  Scores, softmax and sums are float32, keys and values the pages'
  * numbers as they are.  Replays of recordings that use one cache must not overlap. */
 int shainet_attn_attend_paged(shainet_attn_ctx *ctx, shainet_paged_cache *cache, int layer, const int *row_seqs,
                               const int *positions, int rows, const float *q_rot, long long q_stride, float *out,

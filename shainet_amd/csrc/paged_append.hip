@@ -1,6 +1,11 @@
 // bias -> per-head QK-RMSNorm -> half-split RoPE of new rows, as prep_kernel.hip does them (the same arithmetic in the same
 // order, so rows in float32 pages are bit-identical to those of a shainet_kv_cache), with the K and V rows put where a map of
 // slots says and rounded to the pages' type there, once, to the nearest (ties to even).
+//
+// Bound by the rows' bytes where there are many (2048 rows of 32 heads of 128 on 8 kv heads into bfloat16 pages: 46 MB in 9.3 us,
+// as fast as a copy), by a launch and two trips to memory, slot and row, where there are few (333 rows 4.0 us, 16 rows with QK-norm 5.3),
+// and with QK-norm by the squares of a row, which are added one after the other as the contiguous cache's are: 1400 rows 28 us | 12.8
+// without.
 // This file is compiled with -ffp-contract=off: no product may fuse into an add.
 #include "paged.hpp"
 #include "prep_math.hpp"
@@ -101,7 +106,7 @@ __global__ __launch_bounds__(256) void paged_rows_kernel(PrepArgs a, PagePool p,
   }
 }
 
-// Many rows without QK-norm: a lane takes four neighbouring pairs of a head row with 16-byte accesses.
+// Many head rows without QK-norm: a lane takes four neighbouring pairs of a head row with 16-byte accesses.
 __global__ __launch_bounds__(256) void paged_rows_vec_kernel(PrepArgs a, PagePool p, int H, const int *__restrict__ slots,
                                                              const int *__restrict__ positions, int rope_positions,
                                                              long long n_items) {
@@ -217,14 +222,18 @@ hipError_t launch_paged_append(const PrepArgs &a, const PagePool &p, int H, cons
   const bool vec = !a.q_norm && !a.k_norm && ((a.q_stride | a.k_stride | a.v_stride) & 3) == 0 && aligned16(a.q) && aligned16(a.k) &&
                    aligned16(a.v) && aligned16(a.q_rot) && aligned16(p.k) && aligned16(p.v) && aligned16(a.b_q) && aligned16(a.b_k) &&
                    aligned16(a.b_v) && aligned16(a.rope_tab);
-  if (vec && n_rows >= 8192) {
+  // Few head rows take a wavefront each.  Of many, four pairs a lane move the bytes in fewer requests, and 16 rows in LDS add up their
+  // squares side by side.  us a call, 48 head rows of 128 a token: without QK-norm 700 tokens 9.3 | 6.7 by four pairs, 170 as good; with
+  // it 85 tokens 7.0 | 8.1 by LDS, 170 10.7 | 8.8, 1400 60 | 28.
+  constexpr int kFewRows = 6144;
+  if (vec && n_rows >= kFewRows) {
     const long long n_items = n_rows * (p.hd >> 3), blocks = (n_items + 255) / 256;
     if (blocks > 0x7fffffffLL) return hipErrorInvalidValue;
     hipLaunchKernelGGL(paged_rows_vec_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, a, p, H, slots, positions,
                        rope_positions, n_items);
     return hipGetLastError();
   }
-  if (p.hd <= 128 && n_rows < 8192 && rows <= 65535) {
+  if (p.hd <= 128 && n_rows < kFewRows && rows <= 65535) {
     hipLaunchKernelGGL(paged_rows_kernel, dim3((unsigned)((per_token + 3) / 4), (unsigned)rows), dim3(256), 0, stream, a, p, H, slots,
                        positions, rope_positions);
     return hipGetLastError();

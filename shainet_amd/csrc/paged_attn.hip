@@ -492,19 +492,20 @@ __global__ __launch_bounds__((64 * Tile<DTYPE, HD>::WAVES), (Tile<DTYPE, HD>::WA
       for (int i = t; i < a.H * hd; i += THREADS) a.out[r * a.out_stride + i] = 0.0f;
   const long long total = (long long)row_tiles * pairs, n_pairs = (long long)some * pairs;
   int mode = kSpans;
-  const long long share = (total + wgs - 1) / wgs;
-  long long unit = max(1LL, (total + kBegin * n_pairs + wgs - 1) / wgs);  // of a span; or tiles of a chunk, at most
+  int unit = 1;  // tiles and beginnings of a span, or tiles of a chunk at most (32 bits: half a microsecond of a short launch)
   if (n_pairs > wgs && most <= kWavefrontTiles) {
     mode = kWavefronts;
-  } else if (share < kShortSpan && n_pairs <= wgs) {
+  } else if (total <= (long long)wgs * (kShortSpan - 1) && n_pairs <= wgs) {
     // chunks of pairs, one a workgroup: sum of ceil(tiles / unit) <= total / unit + pairs
     mode = kChunks;
-    unit = n_pairs < wgs && most > T::WHOLE ? max((long long)quotient(total + (wgs - n_pairs) - 1, wgs - n_pairs), (long long)WAVES) : most;
+    unit = n_pairs < wgs && most > T::WHOLE ? max(quotient(total + (wgs - n_pairs) - 1, wgs - n_pairs), WAVES) : most;
+  } else {
+    unit = max(1, (int)((total + kBegin * n_pairs + wgs - 1) / wgs));
   }
   if (mode != kWavefronts) {  // units of one kv head before each row
     auto units_of = [&](int r) {
       const int tiles = tiles_of(known_length(r));
-      return mode == kSpans ? (tiles > 0 ? tiles + kBegin : 0) : quotient(tiles + unit - 1, unit);
+      return mode == kSpans ? (tiles > 0 ? tiles + kBegin : 0) : quotient((long long)tiles + unit - 1, unit);
     };
     if (few) {
       const int mine = lane < a.rows ? units_of(lane) : 0, upto = sum_lanes(mine);
@@ -529,7 +530,7 @@ __global__ __launch_bounds__((64 * Tile<DTYPE, HD>::WAVES), (Tile<DTYPE, HD>::WA
   }
 
   const long long all_units = mode == kWavefronts ? (long long)a.rows * pairs : (long long)same(starts[a.rows]) * pairs;
-  long long at = mode == kSpans ? blockIdx.x * unit : mode == kChunks ? blockIdx.x : blockIdx.x + (long long)wgs * wave;
+  long long at = mode == kSpans ? (long long)blockIdx.x * unit : mode == kChunks ? blockIdx.x : blockIdx.x + (long long)wgs * wave;
   const long long end = mode == kSpans ? min(all_units, at + unit) : mode == kChunks ? min(all_units, at + 1) : all_units;
   unsigned *tickets = (unsigned *)a.workspace;
   float *parts = (float *)(tickets + kTickets);
@@ -590,8 +591,8 @@ __global__ __launch_bounds__((64 * Tile<DTYPE, HD>::WAVES), (Tile<DTYPE, HD>::WA
         if (s.last <= s.first) continue;
         s.first_wg = quotient(first_tile, unit);
         s.last_wg = quotient(begins + units - 1, unit);
-        s.late = first_tile > blockIdx.x * unit;
-        s.first_late = first_tile > s.first_wg * unit;
+        s.late = first_tile > (long long)blockIdx.x * unit;
+        s.first_late = first_tile > (long long)s.first_wg * unit;
       } else {  // equal shares
         s.first = quotient((long long)tiles * from, units);
         s.last = quotient((long long)tiles * (from + 1), units);

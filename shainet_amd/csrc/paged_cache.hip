@@ -199,8 +199,10 @@ int append(shainet_attn_ctx *c, shainet_paged_cache *pc, int layer, const PrepAr
 
 int attend(shainet_attn_ctx *c, shainet_paged_cache *pc, int layer, const int *row_seqs, const int *positions, int rows,
            const float *q, long long q_stride, float *out, long long out_stride) {
-  if (rows * reach_of(pc) >= 1LL << 34)  // (tiles of 16 keys are counted in 32 bits)
-    return fail(SHAINET_HIP_ERR_ARGUMENT, "%d rows of up to %lld keys in one call: their product must stay below 2^34", rows, reach_of(pc));
+  // (tiles of 16 keys are counted in 32 bits, and those of a workgroup's span of all pairs)
+  if (rows * reach_of(pc) >= 1LL << 34 || rows * reach_of(pc) * c->KV * ((c->g + 15) / 16) >= 1LL << 42)
+    return fail(SHAINET_HIP_ERR_ARGUMENT, "%d rows of up to %lld keys in one call: their product must stay below 2^34, and times the kv heads below 2^42",
+                rows, reach_of(pc));
   PagedAttendArgs a;
   a.q = q;
   a.out = out;

@@ -919,3 +919,35 @@ def test_maps_of_many_pages(hip, torch, seq_pages):
             got = np.stack([t[:len(want)].cpu().numpy() for t in rows], 1)
             assert np.array_equal(got, np.array(want).reshape(-1, 3))
             assert all((t[len(want):] == -1).all() for t in rows)
+
+
+def test_more_keys_than_can_be_counted(hip, torch):
+    """Tables wide enough for 2^30 keys: so many rows of so many kv heads in one call are refused."""
+    ctx = _ctx(hip, torch, 1024, 1024, 8)
+    cache = hip.PagedKVCache(ctx, 1, 1024, 1, 2 ** 20 - 1)
+    q = torch.zeros((16, 1024 * 8), device="cuda")
+    rows = torch.zeros(16, dtype=torch.int32, device="cuda")
+    for n in (16, 15, 5):
+        with pytest.raises(hip.ArgumentError, match="2\\^42"):
+            ctx.attend_paged(cache, rows[:n], rows[:n], q[:n])
+    out = ctx.attend_paged(cache, rows[:3], rows[:3], q[:3])
+    ctx.sync()
+    assert (out == 0).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("H,KV,hd,n,rows", [(8, 8, 64, 16, 16), (16, 8, 128, 31, 31), (8, 8, 64, 39, 39), (16, 8, 96, 64, 64), (8, 8, 72, 65, 65), (8, 4, 128, 20, 200),
+                                            (4, 2, 256, 30, 90)])
+def test_spans_of_uneven_sequences(hip, torch, H, KV, hd, n, rows, dtype):
+    """Lengths from nothing to some thousand keys: spans that begin and end anywhere, at pairs' ends, behind short ones, within one."""
+    rng = np.random.default_rng(1000 * n + hd)
+    ctx = _ctx(hip, torch, H, KV, hd)
+    for turn in range(3):
+        lens = np.exp(rng.uniform(0, np.log((300, 1200, 4000)[turn]), n)).astype(int) - (rng.random(n) < 0.1)
+        cache, held = _filled(hip, torch, ctx, lens.tolist(), 16, dtype, rng, poison=float("nan"))
+        q = rng.standard_normal((rows, H * hd)).astype(np.float32)
+        seqs = (np.arange(rows) % n).tolist()
+        positions = [int(lens[s]) - 1 - int(rng.integers(0, 3)) * (r >= n) for r, s in enumerate(seqs)]
+        got = ctx.attend_paged(cache, _ints(torch, seqs), _ints(torch, positions), torch.from_numpy(q).cuda())
+        ctx.sync()
+        _check_rows(got.cpu().numpy(), q, held, seqs, [max(p, -1) for p in positions], hd)
