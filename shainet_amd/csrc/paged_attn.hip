@@ -14,7 +14,7 @@
 // waits for anybody.  Short pairs are cut into chunks, one per workgroup, instead, and many short ones go to a wavefront each.
 //
 // Measured (shared rows of all: K and V of 8 kv heads of 128, 32 query heads, pages of 16): 64 sequences of 8192 to 32768 keys of bfloat16
-// 780 us, 6.7 TB/s (8 KiB pieces in any order, 64 KB on their way per compute unit, come at 6.5, 128 KB at 6.8); 16 of 2048 to 8192 of
+// 763 us, 6.8 TB/s (8 KiB pieces in any order, 64 KB on their way per compute unit, come at 6.5, 128 KB at 6.8); 16 of 2048 to 8192 of
 // float32 105 us, 6.2 TB/s; one sequence of 1024 (heads of 64) 9 us, of which an empty launch takes 4.
 //
 // A wavefront has one tile in registers: it asks for the next tile's K once the scores are made, and for its V once the outputs are,
@@ -82,6 +82,8 @@ constexpr int kWavefrontTiles = 16;
 // Tiles that the beginning of a pair costs a workgroup: 39 sequences of up to 5000 keys (bfloat16) 64 us | 86 with none; with 8, 65.  Where all
 // are as long it costs a little: 16 of 500 (float32) 19 us | 17.8.
 constexpr int kBegin = 4;
+// Tiles of a pair, on average, that are many (launch_attend).
+constexpr int kLongPair = 40;
 
 // What is laid out how for pages of a type and heads of up to HD.
 template <int DTYPE, int HD>
@@ -96,6 +98,7 @@ struct Tile {
   static constexpr int WORDS = VEC * E / 4;                // of 4 bytes, in one
   static constexpr int PARTS = DTYPE == kPageF32 ? 1 : DTYPE == kPageBf16 ? 3 : 2;  // of a float operand
   static constexpr int WAVES = 4;                          // of a workgroup
+  static constexpr int LONG = HD == 64 ? 160 : 40;         // tiles of a span that one workgroup on a compute unit reads faster than two
   // Tiles of a pair that is not worth being cut: one sequence of 100 keys (7 tiles of float32) 6.7 us | cut 8.4.
   static constexpr int WHOLE = 12;
 };
@@ -435,7 +438,7 @@ __global__ __launch_bounds__((64 * Tile<DTYPE, HD>::WAVES), (Tile<DTYPE, HD>::WA
   const int hd = PAD ? p.hd : HD;
   const int g = a.g, per_kv = (g + kCols - 1) / kCols, pairs = p.KV * per_kv;
   const int most_keys = (int)min((long long)p.seq_pages << p.shift, 0x3fffffffLL);
-  constexpr int wgs = 256 * PER_CU;  // of every launch
+  constexpr int all_wgs = 256 * PER_CU;  // of every launch
 
   // rows of a length that has a sequence; -1: a row to be left alone
   auto length_of = [&](int r, int &seq) {
@@ -487,10 +490,13 @@ __global__ __launch_bounds__((64 * Tile<DTYPE, HD>::WAVES), (Tile<DTYPE, HD>::WA
   some = same(some);
   most = same(most);
   // outputs of rows without keys
-  for (int r = blockIdx.x; r < a.rows; r += wgs)
+  for (int r = blockIdx.x; r < a.rows; r += all_wgs)
     if (known_length(r) == 0)
       for (int i = t; i < a.H * hd; i += THREADS) a.out[r * a.out_stride + i] = 0.0f;
   const long long total = (long long)row_tiles * pairs, n_pairs = (long long)some * pairs;
+  // Of long spans of long pairs one workgroup on a compute unit is enough, and the others leave (see launch_attend)
+  const int wgs = PER_CU == 2 && total >= (long long)all_wgs * T::LONG && total >= n_pairs * kLongPair ? all_wgs / 2 : all_wgs;
+  if ((int)blockIdx.x >= wgs) return;
   int mode = kSpans;
   int unit = 1;  // tiles and beginnings of a span, or tiles of a chunk at most (32 bits: half a microsecond of a short launch)
   if (n_pairs > wgs && most <= kWavefrontTiles) {
@@ -610,7 +616,7 @@ __global__ __launch_bounds__((64 * Tile<DTYPE, HD>::WAVES), (Tile<DTYPE, HD>::WA
   // 77 to 100 us and the others at 108 to 118 (16 sequences of 2048 to 8192 keys, float32, two on each).  The others' instructions
   // go first, therefore: half to one per cent of most launches.  (Spans of unequal lengths, or short ones for whoever is
   // ready, cost more in parts of pairs than they gave: 110 -> 113 and 121 us.)
-  if (PER_CU == 2 && (int)blockIdx.x >= wgs / 2) __builtin_amdgcn_s_setprio(3);
+  if (PER_CU == 2 && (int)blockIdx.x >= all_wgs / 2) __builtin_amdgcn_s_setprio(3);
   Wave<DTYPE, HD, PAD> w(p, a.scale);
   const bool alone = mode == kWavefronts;
   const int step = alone ? 1 : WAVES, mine = alone ? 0 : wave;
@@ -877,8 +883,10 @@ hipError_t launch_attend(const PagedAttendArgs &a, const PagePool &p, hipStream_
 // One workgroup on a compute unit reads long stretches of few pairs faster than two, of which the first gets ahead: 16 sequences of 2048 to
 // 8192 keys (128 pairs, float32) 105.5 us | two 106.7, one of 131072 (4 pairs, bfloat16) 50 | 53, 24 of 20 to 700 (192 pairs) 10.9 | 12.1.
 // Where there are more pairs than compute units two hide each other's beginnings and ends: 64 sequences of 100 to 300 keys
-// (512 pairs, float32) two 25 us | one 33, 39 of up to 5000 (312 pairs of heads of 64) 38 | 46.  (512 long pairs would like one: 64 of 8192
-// to 32768 keys 766 us | 781; how long they are is known on the device only.)
+// (512 pairs, float32) two 25 us | one 33, 39 of up to 5000 (312 pairs of heads of 64, tiles of half the bytes) 38 | 46.  How long their
+// spans are is known on the device only, where half of the workgroups leave if they are long: 64 sequences of 8192 to 32768 keys
+// (bfloat16) 763 us | two 780, 77 of up to 5000 (heads of 96, float16) 66 | 68.5, 100 of 1000 to 3000 (bfloat16) 132 | 137.  Where
+// pairs are short two are better whatever the spans: 128 of 1000 (32 tiles of bfloat16) 86 us | one 89, 700 of 100 to 700 228 | 257.
 template <int DTYPE, int HD>
 hipError_t launch_attend(const PagedAttendArgs &a, const PagePool &p, hipStream_t stream) {
   if constexpr (HD == 256) {  // (registers for one)
