@@ -951,3 +951,24 @@ def test_spans_of_uneven_sequences(hip, torch, H, KV, hd, n, rows, dtype):
         got = ctx.attend_paged(cache, _ints(torch, seqs), _ints(torch, positions), torch.from_numpy(q).cuda())
         ctx.sync()
         _check_rows(got.cpu().numpy(), q, held, seqs, [max(p, -1) for p in positions], hd)
+
+
+@pytest.mark.parametrize("shift", [0, 1])
+@pytest.mark.parametrize("P", [8, 32])
+def test_maps_of_more_rows_than_threads(hip, torch, P, shift):
+    """Entries of no rows, of a few and of hundreds next to each other, in lists that begin on 16 bytes or do not."""
+    rng = np.random.default_rng(P)
+    n, room = 4096, 480001
+    cache, model = hip.PagedKVCache(_ctx(hip, torch, 1, 1, 8), 60000, P, n, 80), Pages(60000, P, n, 80)
+    for turn in range(3):
+        entries = [(s, min(int(d), 80 * P - model.lens[s])) for s, d in
+                   zip(rng.permutation(n).tolist(), rng.choice([0, 1, 2, 3, 5, 9, 70, 150, -2, -40], n))]
+        entries = [(s, max(d, -model.lens[s])) for s, d in entries]
+        lists = [torch.full((room + shift,), -7, dtype=torch.int32, device="cuda")[shift:] for _ in range(3)]
+        want = np.full((room, 3), -1)
+        rows = model.map(entries, room)
+        want[:len(rows)] = rows
+        cache.map_rows(_ints(torch, [d for _, d in entries]), *lists, seq_ids=_ints(torch, [s for s, _ in entries]))
+        cache.lengths_from_device()
+        _same_state(cache, model, len(model.free))
+        assert np.array_equal(np.stack([t.cpu().numpy() for t in lists], 1), want)
