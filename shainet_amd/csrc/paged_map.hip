@@ -9,8 +9,8 @@
 // the stack as it was, and where a page comes from follows from prefix sums: the order in which threads run decides nothing.
 //
 // Bound by latency: a launch, the entries, their lengths, a table entry or a free page, one after the other.  A step of 16
-// sequences takes 3.9 us on the device (8.7 as one workgroup of 1024 threads that scanned 64-bit sums by shuffles), 582041 rows of
-// 300 prompts 8.4 us (7 MB of lists; 6.8 + 8.1 as two launches, one for the sums and one for the rows).
+// sequences takes 3.3 to 4.0 us on the device (8.7 as one workgroup of 1024 threads that scanned 64-bit sums by shuffles), 582054 rows
+// of 300 prompts 9.3 us (7 MB of lists; as two launches, one for the sums and one for the rows, 15), of which 5.6 without any rows.
 //
 // All or nothing: an entry out of range or named twice, a length below 0 or beyond the table's width, too few pages or
 // too little room for the rows leave everything as it was, with every slot -1 and the reason in *error.
@@ -67,14 +67,20 @@ __device__ __forceinline__ int taken_page(const MapArgs &a, const MapSums &m, in
   return j < m.gone ? pushed_page(a, m, m.gone - 1 - j) : a.free_pages[m.top - 1 - (j - m.gone)];
 }
 
-// Items first, first + step, ...: the pushed pages, the taken ones, the rows.  What is read here (lower stack entries,
-// table entries of pages held) is written by nobody: pushes go above the old top, taken pages into entries beyond the old
-// lengths of other sequences.
+// Items first, first + step, ... of the rows, the pages pushed behind them and the pages taken behind those, so that a thread
+// has one of the three where there are threads enough (1000 sequences, 127644 rows gained and others lost, and the inverse 16.5 us
+// a pair of calls | 20.4 with the three one after the other).  What is read here (lower stack entries, table entries of pages
+// held) is written by nobody: pushes go above the old top, taken pages into entries beyond the old lengths of other sequences.
 template <int EACH>
 __device__ void move_pages(const MapArgs &a, const MapSums &m, int first, int step) {
+  // Of more rows than threads each takes four neighbours, of which one is searched for and most are of one page: 300 prompts of 582054 rows
+  // and their inverse 15.1 us a pair of calls | 16.4.
+  const bool fours = EACH > 1 && a.max_rows > step && (((uintptr_t)a.slots | (uintptr_t)a.positions | (uintptr_t)a.row_seqs) & 15) == 0;
   if (m.ok) {
-    for (int i = first; i < m.gone; i += step) a.free_pages[m.top + i] = pushed_page(a, m, i);
-    for (int j = first; j < m.taken; j += step) {
+    const unsigned row_items = fours ? (a.max_rows + 3u) / 4 : a.max_rows;
+    auto behind = [&](unsigned items) { return first - (int)(items % (unsigned)step) + (first < (int)(items % (unsigned)step) ? step : 0); };
+    for (int i = behind(row_items); i < m.gone; i += step) a.free_pages[m.top + i] = pushed_page(a, m, i);
+    for (int j = behind(row_items + m.gone); j < m.taken; j += step) {
       const int e = entry_of(m.taken_start, m.n, j);
       a.table[(long long)m.seq[e] * a.seq_pages + pages_of(m.old_len[e], a.shift) + (j - m.taken_start[e])] = taken_page(a, m, j);
     }
@@ -85,9 +91,7 @@ __device__ void move_pages(const MapArgs &a, const MapSums &m, int first, int st
     const int had = pages_of(m.old_len[e], a.shift);
     return p < had ? a.table[(long long)m.seq[e] * a.seq_pages + p] : taken_page(a, m, m.taken_start[e] + (p - had));
   };
-  // Of more rows than threads each takes four neighbours, of which one is searched for and most are of one page: 300 prompts of 582041 rows
-  // and their inverse 15.1 us a pair of calls | 16.4.
-  if (EACH > 1 && a.max_rows > step && (((uintptr_t)a.slots | (uintptr_t)a.positions | (uintptr_t)a.row_seqs) & 15) == 0) {
+  if (fours) {
     for (long long r = 4LL * first; r < a.max_rows; r += 4LL * step) {
       int slot[4], pos[4], seq[4], e = -1, of = -1, page = -1;  // (page `of` of entry e)
 #pragma unroll
@@ -288,7 +292,7 @@ hipError_t launch_page_map(const MapArgs &a, hipStream_t stream) {
   if (a.n <= 256 && a.max_rows <= 1024 && pages <= 1 << 16) {
     hipLaunchKernelGGL(page_map_kernel<256>, dim3(1), dim3(256), 0, stream, a);
   } else {
-    const int items = a.max_rows > pages ? a.max_rows : pages, blocks = (items + 1023) / 1024;
+    const long long blocks = ((long long)a.max_rows + pages + 1023) / 1024;
     hipLaunchKernelGGL(page_map_kernel<1024>, dim3((unsigned)(blocks < 1 ? 1 : blocks < 256 ? blocks : 256)), dim3(1024), 0, stream, a);
   }
   return hipGetLastError();
