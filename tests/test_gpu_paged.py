@@ -972,3 +972,24 @@ def test_maps_of_more_rows_than_threads(hip, torch, P, shift):
         cache.lengths_from_device()
         _same_state(cache, model, len(model.free))
         assert np.array_equal(np.stack([t.cpu().numpy() for t in lists], 1), want)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("H,KV,hd,rows", [(8, 8, 128, 44), (16, 8, 96, 45), (8, 8, 80, 47), (8, 8, 64, 150)])
+def test_long_spans_of_many_pairs(hip, torch, H, KV, hd, rows, dtype):
+    """Where half of the workgroups leave: rows by the dozen that share a few long sequences, and some that have next to nothing."""
+    rng = np.random.default_rng(rows)
+    ctx = _ctx(hip, torch, H, KV, hd)
+    lens = [2100, 3990, 3000, 2777, 5]
+    cache, held = _filled(hip, torch, ctx, lens, 32, dtype, rng, poison=float("nan"))
+    seqs = [r % 4 for r in range(rows)]
+    positions = [lens[s] - 1 - r for r, s in enumerate(seqs)]
+    seqs[7], positions[7] = 4, 4
+    seqs[9], positions[9] = 2, -1
+    q = rng.standard_normal((rows, H * hd)).astype(np.float32)
+    args = _ints(torch, seqs), _ints(torch, positions), torch.from_numpy(q).cuda()
+    got = ctx.attend_paged(cache, *args)
+    again = ctx.attend_paged(cache, *args)
+    ctx.sync()
+    _check_rows(got.cpu().numpy(), q, held, seqs, positions, hd)
+    assert torch.equal(got, again)
