@@ -504,7 +504,7 @@ __global__ __launch_bounds__((64 * Tile<DTYPE, HD>::WAVES), (Tile<DTYPE, HD>::WA
   } else if (total <= (long long)wgs * (kShortSpan - 1) && n_pairs <= wgs) {
     // chunks of pairs, one a workgroup: sum of ceil(tiles / unit) <= total / unit + pairs
     mode = kChunks;
-    unit = n_pairs < wgs && most > T::WHOLE ? max(quotient(total + (wgs - n_pairs) - 1, wgs - n_pairs), WAVES) : most;
+    unit = n_pairs < wgs && most > T::WHOLE ? max(quotient(total + (wgs - n_pairs) - 1, wgs - n_pairs), WAVES) : max(most, 1);
   } else {
     unit = max(1, (int)((total + kBegin * n_pairs + wgs - 1) / wgs));
   }

@@ -993,3 +993,18 @@ def test_long_spans_of_many_pairs(hip, torch, H, KV, hd, rows, dtype):
     ctx.sync()
     _check_rows(got.cpu().numpy(), q, held, seqs, positions, hd)
     assert torch.equal(got, again)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", [1, 2, 3, 64, 65, 1000])
+def test_rows_of_which_none_has_a_key(hip, torch, rows, dtype):
+    ctx = _ctx(hip, torch, 8, 2, 64)
+    cache = hip.PagedKVCache(ctx, 4, 8, 3, 2, dtype=dtype)
+    q = torch.randn(rows, 512, device="cuda")
+    seqs = [(0, 2, -1, 3)[r % 4] for r in range(rows)]
+    out = torch.full_like(q, 7)
+    for _ in range(2):
+        ctx.attend_paged(cache, _ints(torch, seqs), _ints(torch, [-1 - r % 5 for r in range(rows)]), q, out)
+    ctx.sync()
+    for r, s in enumerate(seqs):
+        assert (out[r] == (0 if s in (0, 2) else 7)).all(), r
