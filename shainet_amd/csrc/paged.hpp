@@ -4,12 +4,11 @@
 #include <hip/hip_runtime.h>
 
 #include "attn_kernels.hpp"
+#include "paged_tile.hpp"
 
 namespace shainet {
 
-constexpr int kPageF32 = 0, kPageBf16 = 1, kPageF16 = 2;
 constexpr int kMaxPagedSeqs = 4096;  // entries of a map, rows of an attention launch: their prefix sums lie in LDS
-inline int page_element_bytes(int dtype) { return dtype == kPageF32 ? 4 : 2; }
 
 // One layer's pages, [n_pages][KV][1 << shift][hd] for K and for V, and the table of all sequences.
 struct PagePool {

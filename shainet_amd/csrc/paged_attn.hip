@@ -85,17 +85,9 @@ constexpr int kBegin = 4;
 // Tiles of a pair, on average, that are many (launch_attend).
 constexpr int kLongPair = 40;
 
-// What is laid out how for pages of a type and heads of up to HD.
+// ... and what the kernel makes of it.
 template <int DTYPE, int HD>
-struct Tile {
-  static constexpr int E = DTYPE == kPageF32 ? 4 : 2;      // bytes of a number
-  static constexpr int S = DTYPE == kPageF32 ? 1 : 2;      // sixteens of keys of a tile
-  static constexpr int KEYS = 16 * S;
-  static constexpr int CHUNKS = HD * E / 64;               // 16-byte pieces of a K row per lane
-  static constexpr int PER = 16 / E;                       // numbers in one
-  static constexpr int VEC = HD == 96 ? 3 * PER / 4 : HD / 16 < PER ? HD / 16 : PER;  // neighbouring columns of a V row per lane
-  static constexpr int PIECES = HD / (16 * VEC);           // ... how often
-  static constexpr int WORDS = VEC * E / 4;                // of 4 bytes, in one
+struct Tile : PageTile<DTYPE, HD> {
   static constexpr int PARTS = DTYPE == kPageF32 ? 1 : DTYPE == kPageBf16 ? 3 : 2;  // of a float operand
   static constexpr int WAVES = 4;                          // of a workgroup
   static constexpr int LONG = HD == 64 ? 160 : 40;         // tiles of a span that one workgroup on a compute unit reads faster than two
@@ -122,7 +114,7 @@ template <int DTYPE, int HD, bool PAD>
 struct Wave {
   using T = Tile<DTYPE, HD>;
   typedef typename Words<T::WORDS>::T VWords;
-  static constexpr int KEYS_EACH = 4 * T::S;  // of a quarter
+  static constexpr int KEYS_EACH = T::KEYS_EACH;
 
   // A tile in registers, or on its way there.
   struct Held {
@@ -179,24 +171,22 @@ struct Wave {
       const char *row = row_at(k_base, at_page.k, tile * T::KEYS + (m >> 2) * KEYS_EACH + 4 * s + (m & 3));
 #pragma unroll
       for (int u = 0; u < T::CHUNKS; ++u) {
-        int at = (u * 4 + j) * 16;
-        if (PAD) at = at < bytes ? at : 0;
+        const int at = PAD ? T::key_byte(u, j, bytes) : (u * 4 + j) * 16;
         held.k[s][u] = __builtin_nontemporal_load((const u32x4 *)(row + at));
       }
     }
   }
+  // Row `row` of the values' operand, and so of the outputs: the first column of its piece u (or one behind the row's end, which nobody reads)
+  __device__ __forceinline__ int column(int u, int row) const { return PAD && T::RUNS_OVER ? T::value_column(u, row, hd) : T::VEC * (row + 16 * u); }
   __device__ __forceinline__ void ask_v(const Pages &at_page, int tile) {
-    const int bytes = row_bytes();
+    const int numbers = row_bytes() / T::E;
     const char *row = row_at(v_base, at_page.v, tile * T::KEYS + j * KEYS_EACH);
     held.in = (unsigned)at_page.v < (unsigned)p.n_pages;
 #pragma unroll
     for (int r = 0; r < KEYS_EACH; ++r)
 #pragma unroll
-      for (int u = 0; u < T::PIECES; ++u) {
-        int at = (T::VEC * m + 16 * T::VEC * u) * T::E;
-        if (PAD) at = at < bytes ? at : 0;
-        held.v[r][u] = __builtin_nontemporal_load((const VWords *)(row + r * (hd * T::E) + at));
-      }
+      for (int u = 0; u < T::PIECES; ++u)
+        held.v[r][u] = __builtin_nontemporal_load((const VWords *)(row + r * (hd * T::E) + (PAD ? T::value_column(u, m, numbers) : T::VEC * (m + 16 * u)) * T::E));
   }
 
   // The queries as B operands: chunk u of quarter j is d = (4 u + j) PER .. + PER - 1, as K's.
@@ -674,16 +664,14 @@ __global__ __launch_bounds__((64 * Tile<DTYPE, HD>::WAVES), (Tile<DTYPE, HD>::WA
     const float its_sum = sum_across_quarters(w.sum);
     if (alone) {
       const float over = its_sum == 0.0f ? 0.0f : 1.0f / its_sum;
-      if (w.m < cols)
+      if (w.m < cols)  // (columns that two pieces have are the same number twice)
 #pragma unroll
         for (int u = 0; u < T::PIECES; ++u)
 #pragma unroll
           for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int e = 0; e < T::VEC; ++e) {
-              const int d = T::VEC * (4 * w.j + i) + 16 * T::VEC * u + e;
-              if (!PAD || d < hd) out[w.m * hd + d] = w.acc[u][e][i] * over;
-            }
+            for (int e = 0; e < T::VEC; ++e)
+              if (!PAD || T::VEC * (4 * w.j + i + 16 * u) < hd) out[w.m * hd + w.column(u, 4 * w.j + i) + e] = w.acc[u][e][i] * over;
       if (more) put_queries(s);
       continue;
     }
@@ -705,7 +693,7 @@ __global__ __launch_bounds__((64 * Tile<DTYPE, HD>::WAVES), (Tile<DTYPE, HD>::WA
         for (int i = 0; i < 4; ++i)
 #pragma unroll
           for (int e = 0; e < T::VEC; ++e)
-            *outs(wave, w.m, T::VEC * (4 * w.j + i) + 16 * T::VEC * u + e) = w.acc[u][e][i] * fade;
+            *outs(wave, w.m, w.column(u, 4 * w.j + i) + e) = w.acc[u][e][i] * fade;
     if (more) put_largest();
     __syncthreads();
     if (more) put_queries(s);  // (nobody reads the old ones any more)
