@@ -254,8 +254,10 @@ int shainet_paged_cache_map_rows(shainet_paged_cache *cache, const int *seq_ids,
                                  int *positions, int *row_seqs, int max_rows);
 /* After calls that change lengths on the device (map_rows, step_paged) the host's copy is stale and shainet_attn_forward_paged,
  * truncate, read and the two calls for numbers are refused (-1) until this one, which waits.  A replay of such a call is not seen
- * by the host: this one comes after it, too.  (Without it, truncate and forward_paged change nothing, and the next call that
- * waits returns SHAINET_HIP_ERR_ARGUMENT.) */
+ * by the host: this one comes after it, too.  (Without it, truncate and forward_paged, for any layer, change nothing, and the next call that
+ * waits returns SHAINET_HIP_ERR_ARGUMENT.)  Rows that layer 0 mapped before stay good for the layers behind it if nothing but steps' own maps
+ * changed lengths, tables and pages: the device counts the maps, and this call
+ * looks whether the table still has the rows. */
 int shainet_paged_cache_lengths_from_device(shainet_paged_cache *cache);
 int shainet_paged_cache_len(const shainet_paged_cache *cache, int seq);
 int shainet_paged_cache_free_pages(const shainet_paged_cache *cache);
@@ -286,8 +288,9 @@ int shainet_attn_attend_paged(shainet_attn_ctx *ctx, shainet_paged_cache *cache,
                               long long out_stride);
 /* A decode step: one new row for each of n sequences (seq_ids: device array, null: sequences 0..n-1); map, append and attend
  * with lists of the cache's own.  q [n, num_heads*head_dim], k, v [n, num_kv_heads*head_dim], out like q, device pointers.
- * Layer 0 maps the rows; calls for the layers behind it use that map (refused once lengths were changed otherwise).  Can be
- * recorded and replayed.  A step that found no room leaves `out` alone (see map_rows). */
+ * Layer 0 maps the rows; calls for the layers behind it use that map (refused once lengths were changed otherwise; where the host
+ * has not seen that, a replay for instance, they place nothing, leave `out` alone, and the next call that waits returns
+ * SHAINET_HIP_ERR_ARGUMENT).  Can be recorded and replayed.  A step that found no room leaves `out` alone (see map_rows). */
 int shainet_attn_step_paged(shainet_attn_ctx *ctx, shainet_paged_cache *cache, int layer, const int *seq_ids, int n,
                             const float *q, const float *k, const float *v, float *out);
 /* shainet_attn_forward over a cache in pages: any number of new rows for each of up to SHAINET_HIP_MAX_BATCH sequences (host

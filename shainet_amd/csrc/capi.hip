@@ -63,6 +63,10 @@ int check_error_word(int *w) {
     return fail(SHAINET_HIP_ERR_ARGUMENT,
                 "a map of new rows found a sequence out of range or named twice, a length below 0, or one that the host did not know "
                 "(shainet_paged_cache_lengths_from_device): that call changed nothing, and its rows were neither placed nor attended");
+  if (what == kRowsGone)
+    return fail(SHAINET_HIP_ERR_ARGUMENT,
+                "a layer behind the first found that lengths or pages were changed after layer 0 mapped its rows (a replay, or another map): "
+                "they were neither placed nor attended");
   if (what == 2)
     return fail(SHAINET_HIP_ERR_CAPACITY,
                 "a decode step found a sequence at the capacity of its cache or at the end of the context's "

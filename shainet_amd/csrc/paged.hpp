@@ -29,18 +29,31 @@ struct MapArgs {
   int n_seqs, seq_pages, n_pages, shift;
   int *slots, *positions, *row_seqs;  // of the new rows in the entries' order; -1 from the last one to max_rows
   int max_rows;
+  int *epoch;                  // counts the launches that changed something
+  int *rows_epoch;             // nullable: set to the count that the lists are of
   int *scratch;                // a word, zero, which a launch leaves so
   int *error;                  // device-writable: set to kMapNoRoom or kMapBadEntry where nothing was changed
 };
-constexpr int kMapNoRoom = 3, kMapBadEntry = 4;
+constexpr int kMapNoRoom = 3, kMapBadEntry = 4, kRowsGone = 5;
 hipError_t launch_page_map(const MapArgs &a, hipStream_t stream);
 // every length 0, every page free, page 0 to be taken first
-hipError_t launch_page_reset(int *lens, int n_seqs, int *free_pages, int *n_free, int n_pages, hipStream_t stream);
+hipError_t launch_page_reset(int *lens, int n_seqs, int *free_pages, int *n_free, int n_pages, int *epoch, hipStream_t stream);
+// The lengths and, behind them, the first `words` words at a.n_free to `host`, which the device can write to.  Before that counts a change
+// where a.max_rows rows of a map (a.slots, positions, row_seqs; may be none) are not the last ones of their sequences any more, in the slots
+// that the table says.
+hipError_t launch_page_report(const MapArgs &a, int *host, int words, hipStream_t stream);
+
+// Lists that a map for an earlier layer wrote: where lengths, tables or pages were changed since, the rows are nobody's or
+// another's.  Then none is placed, their row_seqs become -1 (so that attention leaves them alone) and *error kRowsGone.
+struct MappedRows {
+  const int *epoch, *rows_epoch;  // (the same word: never)
+  int *row_seqs, *error;
+};
 
 // bias -> QK-norm -> RoPE of `rows` rows, whose K and V parts go to slots[row] (page << shift | row in the page);
 // a.kc, a.vc are not used.  A row whose slot or position is out of range is left alone.
 hipError_t launch_paged_append(const PrepArgs &a, const PagePool &p, int H, const int *slots, const int *positions,
-                               int rope_positions, int rows, hipStream_t stream);
+                               int rope_positions, int rows, const MappedRows &mapped, hipStream_t stream);
 
 // Attention of row r of q ([rows][H * hd], rows q_stride floats apart) over the first positions[r] + 1 rows of sequence
 // row_seqs[r].  A row with row_seqs < 0 is left alone; one with positions < 0 gets zeros.

@@ -29,11 +29,16 @@ struct PagedRow {
 
 // Head row r of a token: the H query heads, then the KV key heads, then the KV value heads.
 __device__ __forceinline__ PagedRow locate(const PrepArgs &a, const PagePool &p, int H, const int *slots, const int *positions,
-                                           int rope_positions, int token, int r) {
+                                           int rope_positions, const MappedRows &mapped, int token, int r) {
   PagedRow rr;
   const int slot = slots[token], hd = p.hd;
+  const bool gone = *mapped.epoch != *mapped.rows_epoch;  // (asked for with the slot: no trip of its own)
   rr.pos = positions[token];
-  rr.valid = r < H + 2 * p.KV && (unsigned)slot < (unsigned)p.n_pages << p.shift && (unsigned)rr.pos < (unsigned)rope_positions;
+  rr.valid = !gone && r < H + 2 * p.KV && (unsigned)slot < (unsigned)p.n_pages << p.shift && (unsigned)rr.pos < (unsigned)rope_positions;
+  if (gone && r == 0) {
+    mapped.row_seqs[token] = -1;
+    *(volatile int *)mapped.error = kRowsGone;
+  }
   rr.rotate = true;
   rr.dtype = kPageF32;
   rr.src = rr.bias = rr.w = nullptr;
@@ -81,9 +86,9 @@ __device__ __forceinline__ void store_quad(void *dst, int dtype, int i, float4 x
 
 // head_dim up to 128: a wavefront per head row, lane i < hd / 2 owns the pair (i, i + hd / 2).
 __global__ __launch_bounds__(256) void paged_rows_kernel(PrepArgs a, PagePool p, int H, const int *__restrict__ slots,
-                                                         const int *__restrict__ positions, int rope_positions) {
+                                                         const int *__restrict__ positions, int rope_positions, MappedRows mapped) {
   const int lane = threadIdx.x & 63, hd = p.hd, half = hd >> 1;
-  const PagedRow rr = locate(a, p, H, slots, positions, rope_positions, blockIdx.y, blockIdx.x * 4 + (threadIdx.x >> 6));
+  const PagedRow rr = locate(a, p, H, slots, positions, rope_positions, mapped, blockIdx.y, blockIdx.x * 4 + (threadIdx.x >> 6));
   if (!rr.valid) return;  // uniform over the wavefront
   const bool active = lane < half;
   const int i = active ? lane : 0;
@@ -109,14 +114,14 @@ __global__ __launch_bounds__(256) void paged_rows_kernel(PrepArgs a, PagePool p,
 // Many head rows without QK-norm: a lane takes four neighbouring pairs of a head row with 16-byte accesses.
 __global__ __launch_bounds__(256) void paged_rows_vec_kernel(PrepArgs a, PagePool p, int H, const int *__restrict__ slots,
                                                              const int *__restrict__ positions, int rope_positions,
-                                                             long long n_items) {
+                                                             MappedRows mapped, long long n_items) {
   const long long idx = (long long)blockIdx.x * 256 + threadIdx.x;
   if (idx >= n_items) return;
   const int half = p.hd >> 1, tpr = half >> 2, rows = H + 2 * p.KV;
   const int j = (int)(idx % tpr);
   const long long row_g = idx / tpr;
   const int token = (int)(row_g / rows);
-  const PagedRow rr = locate(a, p, H, slots, positions, rope_positions, token, (int)(row_g - (long long)token * rows));
+  const PagedRow rr = locate(a, p, H, slots, positions, rope_positions, mapped, token, (int)(row_g - (long long)token * rows));
   if (!rr.valid) return;
   const int i0 = 4 * j;
   float4 x0 = *(const float4 *)(rr.src + i0), x1 = *(const float4 *)(rr.src + half + i0);
@@ -147,7 +152,7 @@ __global__ __launch_bounds__(256) void paged_rows_vec_kernel(PrepArgs a, PagePoo
 template <int ROWS>
 __global__ __launch_bounds__(256) void paged_rows_lds_kernel(PrepArgs a, PagePool p, int H, const int *__restrict__ slots,
                                                              const int *__restrict__ positions, int rope_positions,
-                                                             long long n_rows) {
+                                                             MappedRows mapped, long long n_rows) {
   extern __shared__ float xs[];  // [ROWS][hd + 1]
   __shared__ PagedRow row_s[ROWS];
   __shared__ float inv_s[ROWS];
@@ -158,7 +163,7 @@ __global__ __launch_bounds__(256) void paged_rows_lds_kernel(PrepArgs a, PagePoo
     rr.valid = false;
     if (row_g < n_rows) {
       const int token = (int)(row_g / per_token);
-      rr = locate(a, p, H, slots, positions, rope_positions, token, (int)(row_g - (long long)token * per_token));
+      rr = locate(a, p, H, slots, positions, rope_positions, mapped, token, (int)(row_g - (long long)token * per_token));
     }
     row_s[t] = rr;
   }
@@ -213,7 +218,7 @@ __global__ __launch_bounds__(256) void paged_rows_lds_kernel(PrepArgs a, PagePoo
 }  // namespace
 
 hipError_t launch_paged_append(const PrepArgs &a, const PagePool &p, int H, const int *slots, const int *positions,
-                               int rope_positions, int rows, hipStream_t stream) {
+                               int rope_positions, int rows, const MappedRows &mapped, hipStream_t stream) {
   if (rows <= 0) return hipSuccess;
   if ((p.hd & 7) || p.hd < 8 || p.hd > 256) return hipErrorInvalidValue;
   const int per_token = H + 2 * p.KV;
@@ -230,19 +235,19 @@ hipError_t launch_paged_append(const PrepArgs &a, const PagePool &p, int H, cons
     const long long n_items = n_rows * (p.hd >> 3), blocks = (n_items + 255) / 256;
     if (blocks > 0x7fffffffLL) return hipErrorInvalidValue;
     hipLaunchKernelGGL(paged_rows_vec_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, a, p, H, slots, positions,
-                       rope_positions, n_items);
+                       rope_positions, mapped, n_items);
     return hipGetLastError();
   }
   if (p.hd <= 128 && n_rows < kFewRows && rows <= 65535) {
     hipLaunchKernelGGL(paged_rows_kernel, dim3((unsigned)((per_token + 3) / 4), (unsigned)rows), dim3(256), 0, stream, a, p, H, slots,
-                       positions, rope_positions);
+                       positions, rope_positions, mapped);
     return hipGetLastError();
   }
   constexpr int kRows = 16;
   const long long blocks = (n_rows + kRows - 1) / kRows;
   if (blocks > 0x7fffffffLL) return hipErrorInvalidValue;
   hipLaunchKernelGGL(paged_rows_lds_kernel<kRows>, dim3((unsigned)blocks), dim3(256), (size_t)kRows * (p.hd + 1) * sizeof(float),
-                     stream, a, p, H, slots, positions, rope_positions, n_rows);
+                     stream, a, p, H, slots, positions, rope_positions, mapped, n_rows);
   return hipGetLastError();
 }
 

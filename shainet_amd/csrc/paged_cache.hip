@@ -24,8 +24,11 @@ struct shainet_paged_cache {
   int layers, KV, hd, dtype, n_pages, shift, n_seqs, seq_pages;
   size_t layer_bytes;  // of K, and of V
   char *k = nullptr, *v = nullptr;
-  int *table = nullptr, *lens = nullptr, *free_pages = nullptr, *n_free = nullptr;
-  int *pin = nullptr;      // [n_seqs + 1] on its way from the device
+  int *table = nullptr, *lens = nullptr, *free_pages = nullptr;
+  // kWords on the device: the number of free pages; the count of maps that changed something; the counts that the lists of
+  // step and forward calls are of
+  int *n_free = nullptr;
+  int *pin = nullptr;      // [n_seqs + kWords] pinned, which launch_page_report writes
   int *scratch = nullptr;  // a word for maps
   void *workspace = nullptr;
   // steps: allocated with the cache, so that a step allocates nothing
@@ -42,6 +45,8 @@ struct shainet_paged_cache {
 };
 
 namespace {
+
+enum { kFree, kEpoch, kStepEpoch, kForwardEpoch, kWords };
 
 int fail(int code, const char *fmt, ...) {
   char text[512];
@@ -131,6 +136,7 @@ MapArgs map_of(const shainet_paged_cache *pc) {
   a.seq_pages = pc->seq_pages;
   a.n_pages = pc->n_pages;
   a.shift = pc->shift;
+  a.epoch = pc->n_free + kEpoch;
   a.scratch = pc->scratch;
   a.error = pc->ctx->error;
   return a;
@@ -151,6 +157,7 @@ int map_listed(shainet_paged_cache *pc, const int *ids, const int *was, const in
     a.slots = rows;
     a.positions = rows + max_rows;
     a.row_seqs = rows + 2 * (size_t)max_rows;
+    a.rows_epoch = pc->n_free + kForwardEpoch;
   }
   const hipError_t e = launch_page_map(a, pc->ctx->stream);
   return e == hipSuccess ? SHAINET_HIP_OK : hip_fail(e, "map launch");
@@ -191,9 +198,12 @@ PrepArgs prep_of(const shainet_attn_ctx *c, const float *q, long long q_stride, 
   return pa;
 }
 
+// row_seqs: of rows that a map for layer 0 made, whose count is the word `of_map`; null: the caller's own lists, or just mapped
 int append(shainet_attn_ctx *c, shainet_paged_cache *pc, int layer, const PrepArgs &pa, const int *slots, const int *positions,
-           int rows) {
-  const hipError_t e = launch_paged_append(pa, pool_of(pc, layer), c->H, slots, positions, c->rope_positions, rows, c->stream);
+           int rows, int *row_seqs, int of_map) {
+  const int *epoch = pc->n_free + kEpoch;
+  const MappedRows mapped = {epoch, row_seqs ? pc->n_free + of_map : epoch, row_seqs, pc->ctx->error};
+  const hipError_t e = launch_paged_append(pa, pool_of(pc, layer), c->H, slots, positions, c->rope_positions, rows, mapped, c->stream);
   return e == hipSuccess ? SHAINET_HIP_OK : hip_fail(e, "append launch");
 }
 
@@ -271,8 +281,8 @@ int shainet_paged_cache_create(shainet_paged_cache **out, shainet_attn_ctx *ctx,
   if (e == hipSuccess) e = hipMalloc((void **)&pc->table, table * sizeof(int));
   if (e == hipSuccess) e = hipMalloc((void **)&pc->lens, n_seqs * sizeof(int));
   if (e == hipSuccess) e = hipMalloc((void **)&pc->free_pages, (size_t)n_pages * sizeof(int));
-  if (e == hipSuccess) e = hipMalloc((void **)&pc->n_free, sizeof(int));
-  if (e == hipSuccess) e = hipHostMalloc((void **)&pc->pin, (n_seqs + 1) * sizeof(int), hipHostMallocDefault);
+  if (e == hipSuccess) e = hipMalloc((void **)&pc->n_free, kWords * sizeof(int));
+  if (e == hipSuccess) e = hipHostMalloc((void **)&pc->pin, (n_seqs + kWords) * sizeof(int), hipHostMallocDefault);
   if (e == hipSuccess) e = hipMalloc((void **)&pc->scratch, sizeof(int));
   if (e == hipSuccess) e = hipMalloc(&pc->workspace, ws);
   if (e == hipSuccess) e = hipMalloc((void **)&pc->step_slots, n_seqs * sizeof(int));
@@ -284,7 +294,8 @@ int shainet_paged_cache_create(shainet_paged_cache **out, shainet_attn_ctx *ctx,
   if (e == hipSuccess) e = hipMemsetAsync(pc->table, 0xff, table * sizeof(int), ctx->stream);
   if (e == hipSuccess) e = hipMemsetAsync(pc->workspace, 0, ws, ctx->stream);
   if (e == hipSuccess) e = hipMemsetAsync(pc->scratch, 0, sizeof(int), ctx->stream);
-  if (e == hipSuccess) e = launch_page_reset(pc->lens, n_seqs, pc->free_pages, pc->n_free, n_pages, ctx->stream);
+  if (e == hipSuccess) e = hipMemsetAsync(pc->n_free, 0, kWords * sizeof(int), ctx->stream);
+  if (e == hipSuccess) e = launch_page_reset(pc->lens, n_seqs, pc->free_pages, pc->n_free, n_pages, pc->n_free + kEpoch, ctx->stream);
   if (e == hipSuccess) e = hipStreamSynchronize(ctx->stream);
   if (e != hipSuccess && !rc) rc = hip_fail(e, "allocation of a cache in pages");
   if (!rc) rc = pc->step_q.reserve((size_t)n_seqs * ctx->H * ctx->hd);
@@ -347,16 +358,32 @@ int shainet_paged_cache_lengths_from_device(shainet_paged_cache *pc) {
   if (!pc) return fail(SHAINET_HIP_ERR_ARGUMENT, "cache is null");
   if (int rc = check_device(pc)) return rc;
   if (int rc = refuse_recording(pc->ctx, "shainet_paged_cache_lengths_from_device")) return rc;
-  HIP_TRY(hipMemcpyAsync(pc->pin, pc->lens, pc->n_seqs * sizeof(int), hipMemcpyDeviceToHost, pc->ctx->stream));
-  HIP_TRY(hipMemcpyAsync(pc->pin + pc->n_seqs, pc->n_free, sizeof(int), hipMemcpyDeviceToHost, pc->ctx->stream));
+  // Rows that other layers may still place: whether they are where they were, whoever wrote to lengths or table.  (Those of a step stay
+  // the device's matter: a replay can have made new ones by the time of the next layer.)
+  MapArgs a = map_of(pc);
+  if (pc->layers > 1 && pc->step_rows) {
+    a.max_rows = pc->step_rows;
+    a.slots = pc->step_slots;
+    a.positions = pc->step_positions;
+    a.row_seqs = pc->step_seqs;
+  } else if (pc->layers > 1 && !pc->last_ids.empty()) {
+    for (int n : pc->last_new) a.max_rows += n;
+    a.slots = (int *)pc->rows.p;
+    a.positions = a.slots + a.max_rows;
+    a.row_seqs = a.slots + 2 * (size_t)a.max_rows;
+  }
+  const int *words = pc->pin + pc->n_seqs;
+  const hipError_t e = launch_page_report(a, pc->pin, kWords, pc->ctx->stream);
+  if (e != hipSuccess) return hip_fail(e, "report launch");
   HIP_TRY(hipStreamSynchronize(pc->ctx->stream));
+  if (words[kEpoch] != words[kForwardEpoch]) pc->last_ids.clear();
   for (int s = 0; s < pc->n_seqs; ++s)
     if (pc->pin[s] < 0 || pc->pin[s] > reach_of(pc))
       return fail(SHAINET_HIP_ERR_RUNTIME, "the device holds length %d for sequence %d", pc->pin[s], s);
-  if (pc->pin[pc->n_seqs] < 0 || pc->pin[pc->n_seqs] > pc->n_pages)
-    return fail(SHAINET_HIP_ERR_RUNTIME, "the device holds %d free pages of %d", pc->pin[pc->n_seqs], pc->n_pages);
+  if (words[kFree] < 0 || words[kFree] > pc->n_pages)
+    return fail(SHAINET_HIP_ERR_RUNTIME, "the device holds %d free pages of %d", words[kFree], pc->n_pages);
   memcpy(pc->len.data(), pc->pin, pc->n_seqs * sizeof(int));
-  pc->free_count = pc->pin[pc->n_seqs];
+  pc->free_count = words[kFree];
   pc->lengths_on_device = false;
   return check_error_word(pc->ctx->error);
 }
@@ -391,7 +418,7 @@ int shainet_paged_cache_clear(shainet_paged_cache *pc, int seq) {
   if (seq >= 0) return shainet_paged_cache_truncate(pc, seq, 0);
   if (int rc = check_device(pc)) return rc;
   if (int rc = refuse_recording(pc->ctx, "shainet_paged_cache_clear")) return rc;
-  const hipError_t e = launch_page_reset(pc->lens, pc->n_seqs, pc->free_pages, pc->n_free, pc->n_pages, pc->ctx->stream);
+  const hipError_t e = launch_page_reset(pc->lens, pc->n_seqs, pc->free_pages, pc->n_free, pc->n_pages, pc->n_free + kEpoch, pc->ctx->stream);
   if (e != hipSuccess) return hip_fail(e, "reset launch");
   pc->len.assign(pc->n_seqs, 0);
   pc->free_count = pc->n_pages;
@@ -429,7 +456,7 @@ int shainet_attn_append_paged(shainet_attn_ctx *c, shainet_paged_cache *pc, int 
   if (q_stride < (long long)c->H * c->hd || k_stride < (long long)c->KV * c->hd || v_stride < (long long)c->KV * c->hd)
     return fail(SHAINET_HIP_ERR_ARGUMENT, "row strides must be at least the row widths %d and %d", c->H * c->hd, c->KV * c->hd);
   if (int rc = reach_table(c, reach_of(pc))) return rc;
-  return append(c, pc, layer, prep_of(c, q, q_stride, k, k_stride, v, v_stride, q_rot), slots, positions, rows);
+  return append(c, pc, layer, prep_of(c, q, q_stride, k, k_stride, v, v_stride, q_rot), slots, positions, rows, nullptr, 0);
 }
 
 int shainet_attn_attend_paged(shainet_attn_ctx *c, shainet_paged_cache *pc, int layer, const int *row_seqs, const int *positions,
@@ -459,6 +486,7 @@ int shainet_attn_step_paged(shainet_attn_ctx *c, shainet_paged_cache *pc, int la
     a.positions = pc->step_positions;
     a.row_seqs = pc->step_seqs;
     a.max_rows = n;
+    a.rows_epoch = pc->n_free + kStepEpoch;
     const hipError_t e = launch_page_map(a, c->stream);
     if (e != hipSuccess) return hip_fail(e, "map launch");
     pc->lengths_on_device = true;
@@ -467,7 +495,9 @@ int shainet_attn_step_paged(shainet_attn_ctx *c, shainet_paged_cache *pc, int la
   }
   const long long q_dim = (long long)c->H * c->hd, kv_dim = (long long)c->KV * c->hd;
   float *q_rot = pc->step_q.p;
-  if (int rc = append(c, pc, layer, prep_of(c, q, q_dim, k, kv_dim, v, kv_dim, q_rot), pc->step_slots, pc->step_positions, n)) return rc;
+  if (int rc = append(c, pc, layer, prep_of(c, q, q_dim, k, kv_dim, v, kv_dim, q_rot), pc->step_slots, pc->step_positions, n,
+                      layer ? pc->step_seqs : nullptr, kStepEpoch))
+    return rc;
   return attend(c, pc, layer, pc->step_seqs, pc->step_positions, n, q_rot, q_dim, out, q_dim);
 }
 
@@ -490,6 +520,7 @@ int shainet_attn_forward_paged(shainet_attn_ctx *c, shainet_paged_cache *pc, int
     if (more < 1) return fail(SHAINET_HIP_ERR_ARGUMENT, "new_tokens must be positive");
     // (layers behind the first: the rows are counted already)
     start[s] = layer == 0 ? pc->len[id] : pc->len[id] - more;
+    if (start[s] < 0) return fail(SHAINET_HIP_ERR_ARGUMENT, "layer %d: other rows than layer 0 had last: sequence %d has %d, not %d new ones", layer, id, pc->len[id], more);
     if ((long long)start[s] + more > reach_of(pc))
       return fail(SHAINET_HIP_ERR_CAPACITY, "sequence %d: %d cached + %d new rows exceed the %lld of its table", id, start[s], more, reach_of(pc));
     pages += pages_of(pc, (long long)start[s] + more) - pages_of(pc, start[s]);
@@ -532,7 +563,8 @@ int shainet_attn_forward_paged(shainet_attn_ctx *c, shainet_paged_cache *pc, int
   }
   if (rc) return rc;
   int *lists = (int *)pc->rows.p;
-  const int *slots = lists, *positions = lists + rows, *row_seqs = lists + 2 * (size_t)rows;
+  const int *slots = lists, *positions = lists + rows;
+  int *row_seqs = lists + 2 * (size_t)rows;
   if (layer == 0) {
     try {
       pc->last_ids.assign(ids, ids + n_seqs);
@@ -548,7 +580,8 @@ int shainet_attn_forward_paged(shainet_attn_ctx *c, shainet_paged_cache *pc, int
     }
   }
   const long long q_dim = (long long)c->H * c->hd, kv_dim = (long long)c->KV * c->hd;
-  rc = append(c, pc, layer, prep_of(c, dq, q_dim, dk, kv_dim, dv, kv_dim, c->q_rot.p), slots, positions, rows);
+  rc = append(c, pc, layer, prep_of(c, dq, q_dim, dk, kv_dim, dv, kv_dim, c->q_rot.p), slots, positions, rows,
+              layer ? row_seqs : nullptr, kForwardEpoch);
   // entries of a few rows each go together, from row `done` on; one of many by itself
   int at = 0, done = 0;
   for (int s = 0; s <= n_seqs && !rc; ++s) {

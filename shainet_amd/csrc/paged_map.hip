@@ -13,7 +13,8 @@
 // of 300 prompts 9.3 us (7 MB of lists; as two launches, one for the sums and one for the rows, 15), of which 5.6 without any rows.
 //
 // All or nothing: an entry out of range or named twice, a length below 0 or beyond the table's width, too few pages or
-// too little room for the rows leave everything as it was, with every slot -1 and the reason in *error.
+// too little room for the rows leave everything as it was, with every slot -1 and the reason in *error.  Launches that change something
+// are counted: rows are placed layer by layer, and a layer behind the first asks by the count whether they are still its sequences'.
 #include "paged.hpp"
 #include "lane_sums.hpp"
 
@@ -149,7 +150,7 @@ __global__ __launch_bounds__(THREADS) void page_map_kernel(MapArgs a) {
   __shared__ unsigned named[kMaxPagedSeqs / 32];
   __shared__ int bad, last;
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6, each = EACH == 1 ? 1 : (a.n + THREADS - 1) / THREADS;
-  const int top = *a.n_free;
+  const int top = *a.n_free, epoch = *a.epoch;
   const long long most = (long long)a.seq_pages << a.shift;
   int id[EACH], change[EACH], old_len[EACH], new_len[EACH];
 #pragma unroll
@@ -263,18 +264,46 @@ __global__ __launch_bounds__(THREADS) void page_map_kernel(MapArgs a) {
   for (int u = 0; u < EACH; ++u)
     if (u < each && t * each + u < a.n && ok) a.lens[id[u]] = new_len[u];
   if (t == 0) {
-    if (ok)
+    if (ok) {
       *a.n_free = top + all[1] - all[2];
-    else
+      *a.epoch = epoch + 1;
+    } else {
       *(volatile int *)a.error = bad & 1 ? kMapBadEntry : kMapNoRoom;
+    }
+    if (a.rows_epoch) *a.rows_epoch = ok ? epoch + 1 : epoch;
   }
 }
 
-__global__ __launch_bounds__(256) void page_reset_kernel(int *lens, int n_seqs, int *free_pages, int *n_free, int n_pages) {
+__global__ __launch_bounds__(1024) void page_report_kernel(MapArgs a, int *host, int words) {
+  const long long most = (long long)a.seq_pages << a.shift;
+  const int in_page = (1 << a.shift) - 1;
+  int gone = 0;
+  for (int r = threadIdx.x; r < a.max_rows; r += 1024) {
+    const int seq = a.row_seqs[r], pos = a.positions[r], slot = a.slots[r];
+    if ((unsigned)seq >= (unsigned)a.n_seqs || pos < 0 || pos >= most) {
+      gone = 1;
+      continue;
+    }
+    // (a sequence's rows follow each other, and the last is its last)
+    const bool ends = r + 1 == a.max_rows || a.row_seqs[r + 1] != seq;
+    if (slot >> a.shift != a.table[(long long)seq * a.seq_pages + (pos >> a.shift)] || (slot & in_page) != (pos & in_page) ||
+        (ends ? a.lens[seq] : a.positions[r + 1]) != pos + 1)
+      gone = 1;
+  }
+  gone = __syncthreads_or(gone);
+  if (threadIdx.x == 0 && gone) *a.epoch += 1;
+  __syncthreads();
+  for (int i = threadIdx.x; i < a.n_seqs + words; i += 1024) host[i] = i < a.n_seqs ? a.lens[i] : a.n_free[i - a.n_seqs];
+}
+
+__global__ __launch_bounds__(256) void page_reset_kernel(int *lens, int n_seqs, int *free_pages, int *n_free, int n_pages, int *epoch) {
   const int i = blockIdx.x * 256 + threadIdx.x;
   if (i < n_seqs) lens[i] = 0;
   if (i < n_pages) free_pages[i] = n_pages - 1 - i;
-  if (i == 0) *n_free = n_pages;
+  if (i == 0) {
+    *n_free = n_pages;
+    *epoch += 1;
+  }
 }
 
 }  // namespace
@@ -298,10 +327,15 @@ hipError_t launch_page_map(const MapArgs &a, hipStream_t stream) {
   return hipGetLastError();
 }
 
-hipError_t launch_page_reset(int *lens, int n_seqs, int *free_pages, int *n_free, int n_pages, hipStream_t stream) {
+hipError_t launch_page_report(const MapArgs &a, int *host, int words, hipStream_t stream) {
+  hipLaunchKernelGGL(page_report_kernel, dim3(1), dim3(1024), 0, stream, a, host, words);
+  return hipGetLastError();
+}
+
+hipError_t launch_page_reset(int *lens, int n_seqs, int *free_pages, int *n_free, int n_pages, int *epoch, hipStream_t stream) {
   const int items = n_seqs > n_pages ? n_seqs : n_pages;
   hipLaunchKernelGGL(page_reset_kernel, dim3((unsigned)((items + 255) / 256)), dim3(256), 0, stream, lens, n_seqs, free_pages,
-                     n_free, n_pages);
+                     n_free, n_pages, epoch);
   return hipGetLastError();
 }
 
