@@ -516,42 +516,65 @@ class AttnContext:
 
         return call
 
+    # Memory for outputs belongs to torch's current stream, which may still use it for something else and takes it back as soon as
+    # nobody holds the tensor.  A context on another stream waits for the current one before it writes there, and the current
+    # one for it afterwards (on the device: no waiting here).
+
+    def _join(self):
+        """The context's stream, which now waits for torch's current one, if it is another; None where they are the same."""
+        import torch
+
+        own = self.stream or 0
+        if torch.cuda.current_stream().cuda_stream == own:
+            return None
+        there = torch.cuda.ExternalStream(own)
+        there.wait_stream(torch.cuda.current_stream())
+        return there
+
+    @staticmethod
+    def _leave(there):
+        if there is not None:
+            import torch
+
+            torch.cuda.current_stream().wait_stream(there)
+
     # The calls of a decode step are made hundreds of times a second and each takes a few microseconds on the device: their
     # checks look at every argument once and nothing else is done (append_paged: 10.3 us a call, 6 of them checks, before).
 
     def append_paged(self, cache, slots, positions, q, k, v, q_rot=None, layer=0):
         """shainet_attn_append_paged: bias, QK-norm and rotation of rows of q, k and v (torch CUDA float32, rows may be
         strided); K and V rows into slots[row] of a `PagedKVCache`, rotated queries into q_rot.  slots and positions are
-        int32 CUDA tensors, as `PagedKVCache.map_rows` writes them."""
-        dev = cache._device
+        int32 CUDA tensors, as `PagedKVCache.map_rows` writes them.  Without q_rot, streams wait for each other where the
+        context's is not torch's current one."""
+        dev, there = cache._device, None
         rows = _ints(slots, dev)
         _ints(positions, dev, rows)
         qs, ks, vs = _rows(q, dev, rows, self.q_dim), _rows(k, dev, rows, self.kv_dim), _rows(v, dev, rows, self.kv_dim)
         if q_rot is None:
-            q_rot = q.new_empty((rows, self.q_dim))
+            q_rot, there = q.new_empty((rows, self.q_dim)), self._join()
         elif _rows(q_rot, dev, rows, self.q_dim) != self.q_dim:
             raise ArgumentError("q_rot must be contiguous")
         rc = _lib.shainet_attn_append_paged(self._h, cache._h, layer, slots.data_ptr(), positions.data_ptr(), rows, q.data_ptr(), qs,
                                             k.data_ptr(), ks, v.data_ptr(), vs, q_rot.data_ptr())
+        self._leave(there)
         if rc:
             _check(rc)
         return q_rot
 
     def attend_paged(self, cache, row_seqs, positions, q_rot, out=None, layer=0):
         """shainet_attn_attend_paged: attention of rotated query rows over the first positions[row] + 1 rows of sequence
-        row_seqs[row] of a `PagedKVCache` (int32 CUDA tensors).  Rows whose row_seqs is no sequence are left alone in `out`."""
-        dev = cache._device
+        row_seqs[row] of a `PagedKVCache` (int32 CUDA tensors).  Rows whose row_seqs is no sequence are left alone in `out`, whose
+        place zeros take if there is none (and streams wait for each other, as in append_paged)."""
+        dev, there = cache._device, None
         rows = _ints(row_seqs, dev)
         _ints(positions, dev, rows)
         stride = _rows(q_rot, dev, rows, self.q_dim)
         if out is None:
-            import torch
-
             out = q_rot.new_zeros((rows, self.q_dim))
-            if torch.cuda.current_stream().cuda_stream != (self.stream or 0):
-                torch.cuda.current_stream().synchronize()  # (the zeros of rows left alone are there before the kernel writes)
+            there = self._join()
         rc = _lib.shainet_attn_attend_paged(self._h, cache._h, layer, row_seqs.data_ptr(), positions.data_ptr(), rows, q_rot.data_ptr(),
                                             stride, out.data_ptr(), _rows(out, dev, rows, self.q_dim))
+        self._leave(there)
         if rc:
             _check(rc)
         return out
@@ -572,10 +595,11 @@ class AttnContext:
 
     def forward_paged(self, cache, q, k, v, new_tokens, seq_ids=None, out=None, layer=0):
         """`forward` over a `PagedKVCache`: any number of new rows for each of len(new_tokens) sequences.  numpy inputs run
-        the synchronous host-pointer mode and return numpy; torch CUDA tensors the asynchronous one."""
+        the synchronous host-pointer mode and return numpy; torch CUDA tensors the asynchronous one (without `out`, streams wait
+        for each other, as in append_paged)."""
         import numpy as np
 
-        n, rows = len(new_tokens), sum(new_tokens)
+        n, rows, there = len(new_tokens), sum(new_tokens), None
         nt = (C.c_int * n)(*new_tokens)
         ids = (C.c_int * n)(*seq_ids) if seq_ids is not None else None
         if seq_ids is not None and len(seq_ids) != n:
@@ -588,14 +612,19 @@ class AttnContext:
         else:
             import torch
 
-            if out is None:
+            made = out is None
+            if made:
                 out = torch.empty_like(q)
             dev = cache._device
             for t, width in ((q, self.q_dim), (k, self.kv_dim), (v, self.kv_dim), (out, self.q_dim)):
                 if _rows(t, dev, rows, width) != width:
                     raise ArgumentError("q, k, v and out must be contiguous")
             mem = MEM_DEVICE
-        _check(lib().shainet_attn_forward_paged(self._h, cache._h, layer, ids, nt, n, _ptr(q), _ptr(k), _ptr(v), _ptr(out), mem))
+            if made:
+                there = self._join()
+        rc = lib().shainet_attn_forward_paged(self._h, cache._h, layer, ids, nt, n, _ptr(q), _ptr(k), _ptr(v), _ptr(out), mem)
+        self._leave(there)
+        _check(rc)
         return out
 
 
