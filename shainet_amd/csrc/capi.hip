@@ -57,8 +57,8 @@ int check_error_word(int *w) {
   *(volatile int *)w = 0;
   if (what == kMapNoRoom)
     return fail(SHAINET_HIP_ERR_CAPACITY,
-                "a map of new rows found too few free pages, a sequence at the end of its table or more rows than the caller's "
-                "lists hold: that call changed nothing, and its rows were neither placed nor attended");
+                "a map of new rows found too few free pages, a sequence at the end of its table or of the context's cos/sin table, or more "
+                "rows than the caller's lists hold: that call changed nothing, and its rows were neither placed nor attended");
   if (what == kMapBadEntry)
     return fail(SHAINET_HIP_ERR_ARGUMENT,
                 "a map of new rows found a sequence out of range or named twice, a length below 0, or one that the host did not know "
@@ -67,6 +67,10 @@ int check_error_word(int *w) {
     return fail(SHAINET_HIP_ERR_ARGUMENT,
                 "a layer behind the first found that lengths or pages were changed after layer 0 mapped its rows (a replay, or another map): "
                 "they were neither placed nor attended");
+  if (what == kRowsFar)
+    return fail(SHAINET_HIP_ERR_CAPACITY,
+                "a layer behind the first found rows behind the end of its context's cos/sin table (shainet_paged_cache_lengths_from_device "
+                "lets the next call extend it): they were neither placed nor attended");
   if (what == 2)
     return fail(SHAINET_HIP_ERR_CAPACITY,
                 "a decode step found a sequence at the capacity of its cache or at the end of the context's "

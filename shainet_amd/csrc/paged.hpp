@@ -25,29 +25,31 @@ struct MapArgs {
   const int *ids, *delta;      // device; null: see `inlined`, else sequence i and one row
   int inlined;                 // the lists below instead, n <= kMaxSeqs; a sequence whose length is not `was` is a bad entry
   int id[kMaxSeqs], was[kMaxSeqs], change[kMaxSeqs];
-  int *table, *lens, *free_pages, *n_free;
+  int *table, *lens, *free_pages;
+  int *n_free;                 // and, behind it, the count of launches that changed something; on 8 bytes
   int n_seqs, seq_pages, n_pages, shift;
+  int reach;                   // entries that grow become no longer than this
   int *slots, *positions, *row_seqs;  // of the new rows in the entries' order; -1 from the last one to max_rows
   int max_rows;
-  int *epoch;                  // counts the launches that changed something
   int *rows_epoch;             // nullable: set to the count that the lists are of
   int *scratch;                // a word, zero, which a launch leaves so
   int *error;                  // device-writable: set to kMapNoRoom or kMapBadEntry where nothing was changed
 };
-constexpr int kMapNoRoom = 3, kMapBadEntry = 4, kRowsGone = 5;
+constexpr int kMapNoRoom = 3, kMapBadEntry = 4, kRowsGone = 5, kRowsFar = 6;
 hipError_t launch_page_map(const MapArgs &a, hipStream_t stream);
 // every length 0, every page free, page 0 to be taken first
-hipError_t launch_page_reset(int *lens, int n_seqs, int *free_pages, int *n_free, int n_pages, int *epoch, hipStream_t stream);
+hipError_t launch_page_reset(int *lens, int n_seqs, int *free_pages, int *n_free, int n_pages, hipStream_t stream);
 // The lengths and, behind them, the first `words` words at a.n_free to `host`, which the device can write to.  Before that counts a change
 // where a.max_rows rows of a map (a.slots, positions, row_seqs; may be none) are not the last ones of their sequences any more, in the slots
 // that the table says.
 hipError_t launch_page_report(const MapArgs &a, int *host, int words, hipStream_t stream);
 
 // Lists that a map for an earlier layer wrote: where lengths, tables or pages were changed since, the rows are nobody's or
-// another's.  Then none is placed, their row_seqs become -1 (so that attention leaves them alone) and *error kRowsGone.
+// another's.  Then none is placed, their row_seqs become -1 (so that attention leaves them alone) and *error kRowsGone; one at a position
+// that this layer's cos/sin table does not have goes the same way, with kRowsFar.
 struct MappedRows {
   const int *epoch, *rows_epoch;  // (the same word: never)
-  int *row_seqs, *error;
+  int *row_seqs, *error;          // row_seqs null: lists of the caller's, or of the map just before
 };
 
 // bias -> QK-norm -> RoPE of `rows` rows, whose K and V parts go to slots[row] (page << shift | row in the page);

@@ -35,9 +35,9 @@ __device__ __forceinline__ PagedRow locate(const PrepArgs &a, const PagePool &p,
   const bool gone = *mapped.epoch != *mapped.rows_epoch;  // (asked for with the slot: no trip of its own)
   rr.pos = positions[token];
   rr.valid = !gone && r < H + 2 * p.KV && (unsigned)slot < (unsigned)p.n_pages << p.shift && (unsigned)rr.pos < (unsigned)rope_positions;
-  if (gone && r == 0) {
+  if (mapped.row_seqs && r == 0 && (gone || rr.pos >= rope_positions)) {
     mapped.row_seqs[token] = -1;
-    *(volatile int *)mapped.error = kRowsGone;
+    *(volatile int *)mapped.error = gone ? kRowsGone : kRowsFar;
   }
   rr.rotate = true;
   rr.dtype = kPageF32;

@@ -40,6 +40,7 @@ struct shainet_paged_cache {
   DevBuf gathered;
   std::vector<int> len;    // per sequence, while the host knows them
   int free_count;
+  int reach;               // rows that a sequence may come to have, as far as the host knows: the context's cos/sin tables go as far
   bool lengths_on_device = false;
   std::vector<int> last_ids, last_new;  // of the last forward call for layer 0
 };
@@ -136,15 +137,21 @@ MapArgs map_of(const shainet_paged_cache *pc) {
   a.seq_pages = pc->seq_pages;
   a.n_pages = pc->n_pages;
   a.shift = pc->shift;
-  a.epoch = pc->n_free + kEpoch;
+  a.reach = (int)reach_of(pc);
   a.scratch = pc->scratch;
   a.error = pc->ctx->error;
   return a;
 }
 
+// Rows that c places have an angle each: maps of rows for its calls refuse those behind its table.
+int reach_with(const shainet_attn_ctx *c, const shainet_paged_cache *pc) {
+  return (int)(c->rope_positions < reach_of(pc) ? c->rope_positions : reach_of(pc));
+}
+
 // The lengths of up to kMaxSeqs sequences, `was` as far as the host knows, change by `change`; rows (nullable): three lists of max_rows.
-int map_listed(shainet_paged_cache *pc, const int *ids, const int *was, const int *change, int n, int *rows, int max_rows) {
+int map_listed(shainet_paged_cache *pc, const int *ids, const int *was, const int *change, int n, int reach, int *rows, int max_rows) {
   MapArgs a = map_of(pc);
+  a.reach = reach;
   a.n = n;
   a.inlined = 1;
   for (int i = 0; i < n; ++i) {
@@ -163,8 +170,16 @@ int map_listed(shainet_paged_cache *pc, const int *ids, const int *was, const in
   return e == hipSuccess ? SHAINET_HIP_OK : hip_fail(e, "map launch");
 }
 
-// Positions that a map of rows can give; a caller's own lists may name any that the table holds.
-long long mapped_reach(const shainet_paged_cache *pc) { return (long long)(pc->seq_pages < pc->n_pages ? pc->seq_pages : pc->n_pages) << pc->shift; }
+constexpr long long kMostTableBytes = 8LL << 30;
+long long most_positions(const shainet_attn_ctx *c) { return kMostTableBytes / ((long long)c->hd * 4); }
+
+// Sequences that hold pages of the pool only, each its own, are no longer than the pool; of those that a caller made longer (entries of
+// no page, pages shared) the host knows once it is told their lengths.
+void extend_reach(shainet_paged_cache *pc, long long rows) {
+  if (rows <= pc->reach) return;
+  const long long most = most_positions(pc->ctx), more = 2 * rows < most ? 2 * rows : rows < most ? most : rows;
+  pc->reach = (int)(more < reach_of(pc) ? more : reach_of(pc));
+}
 
 // The cos/sin table goes as far as rows can: at which positions they are is known to the device only.
 int reach_table(shainet_attn_ctx *c, long long reach) {
@@ -172,7 +187,7 @@ int reach_table(shainet_attn_ctx *c, long long reach) {
   if (refuse_recording(c, ""))
     return fail(SHAINET_HIP_ERR_ARGUMENT, "the context's cos/sin table must be extended to %lld positions, which cannot be recorded: create the context "
                 "with that many, or place rows once before recording", reach);
-  if (reach * c->hd * 4 > 8LL << 30)
+  if (reach > most_positions(c))
     return fail(SHAINET_HIP_ERR_ALLOC, "a cos/sin table of %lld positions would take more than 8 GiB: the cache's table is that wide", reach);
   return ensure_rope_table(c, (int)reach);
 }
@@ -267,6 +282,7 @@ int shainet_paged_cache_create(shainet_paged_cache **out, shainet_attn_ctx *ctx,
   pc->n_seqs = n_seqs;
   pc->seq_pages = seq_pages;
   pc->free_count = n_pages;
+  pc->reach = (seq_pages < n_pages ? seq_pages : n_pages) * page_rows;
   pc->layer_bytes = (size_t)n_pages * ctx->KV * page_rows * ctx->hd * page_element_bytes(dtype);
   int rc = SHAINET_HIP_OK;
   try {
@@ -295,7 +311,7 @@ int shainet_paged_cache_create(shainet_paged_cache **out, shainet_attn_ctx *ctx,
   if (e == hipSuccess) e = hipMemsetAsync(pc->workspace, 0, ws, ctx->stream);
   if (e == hipSuccess) e = hipMemsetAsync(pc->scratch, 0, sizeof(int), ctx->stream);
   if (e == hipSuccess) e = hipMemsetAsync(pc->n_free, 0, kWords * sizeof(int), ctx->stream);
-  if (e == hipSuccess) e = launch_page_reset(pc->lens, n_seqs, pc->free_pages, pc->n_free, n_pages, pc->n_free + kEpoch, ctx->stream);
+  if (e == hipSuccess) e = launch_page_reset(pc->lens, n_seqs, pc->free_pages, pc->n_free, n_pages, ctx->stream);
   if (e == hipSuccess) e = hipStreamSynchronize(ctx->stream);
   if (e != hipSuccess && !rc) rc = hip_fail(e, "allocation of a cache in pages");
   if (!rc) rc = pc->step_q.reserve((size_t)n_seqs * ctx->H * ctx->hd);
@@ -377,13 +393,17 @@ int shainet_paged_cache_lengths_from_device(shainet_paged_cache *pc) {
   if (e != hipSuccess) return hip_fail(e, "report launch");
   HIP_TRY(hipStreamSynchronize(pc->ctx->stream));
   if (words[kEpoch] != words[kForwardEpoch]) pc->last_ids.clear();
-  for (int s = 0; s < pc->n_seqs; ++s)
+  int longest = 0;
+  for (int s = 0; s < pc->n_seqs; ++s) {
     if (pc->pin[s] < 0 || pc->pin[s] > reach_of(pc))
       return fail(SHAINET_HIP_ERR_RUNTIME, "the device holds length %d for sequence %d", pc->pin[s], s);
+    if (pc->pin[s] > longest) longest = pc->pin[s];
+  }
   if (words[kFree] < 0 || words[kFree] > pc->n_pages)
     return fail(SHAINET_HIP_ERR_RUNTIME, "the device holds %d free pages of %d", words[kFree], pc->n_pages);
   memcpy(pc->len.data(), pc->pin, pc->n_seqs * sizeof(int));
   pc->free_count = words[kFree];
+  if (longest > pc->reach || (longest == pc->reach && pc->free_count)) extend_reach(pc, (long long)longest + 1);
   pc->lengths_on_device = false;
   return check_error_word(pc->ctx->error);
 }
@@ -406,7 +426,7 @@ int shainet_paged_cache_truncate(shainet_paged_cache *pc, int seq, int len) {
   if (int rc = refuse_recording(pc->ctx, "shainet_paged_cache_truncate")) return rc;
   const int was = pc->len[seq], change = len - was;
   if (change == 0) return SHAINET_HIP_OK;
-  if (int rc = map_listed(pc, &seq, &was, &change, 1, nullptr, 0)) return rc;
+  if (int rc = map_listed(pc, &seq, &was, &change, 1, 0, nullptr, 0)) return rc;
   pc->free_count += pages_of(pc, pc->len[seq]) - pages_of(pc, len);
   pc->len[seq] = len;
   forget_rows(pc);
@@ -418,7 +438,7 @@ int shainet_paged_cache_clear(shainet_paged_cache *pc, int seq) {
   if (seq >= 0) return shainet_paged_cache_truncate(pc, seq, 0);
   if (int rc = check_device(pc)) return rc;
   if (int rc = refuse_recording(pc->ctx, "shainet_paged_cache_clear")) return rc;
-  const hipError_t e = launch_page_reset(pc->lens, pc->n_seqs, pc->free_pages, pc->n_free, pc->n_pages, pc->n_free + kEpoch, pc->ctx->stream);
+  const hipError_t e = launch_page_reset(pc->lens, pc->n_seqs, pc->free_pages, pc->n_free, pc->n_pages, pc->ctx->stream);
   if (e != hipSuccess) return hip_fail(e, "reset launch");
   pc->len.assign(pc->n_seqs, 0);
   pc->free_count = pc->n_pages;
@@ -477,10 +497,11 @@ int shainet_attn_step_paged(shainet_attn_ctx *c, shainet_paged_cache *pc, int la
   if (n < 1 || n > pc->n_seqs) return fail(SHAINET_HIP_ERR_ARGUMENT, "n must be in 1..%d", pc->n_seqs);
   if (layer > 0 && n != pc->step_rows)
     return fail(SHAINET_HIP_ERR_ARGUMENT, "layer %d of a step of %d rows: layer 0 mapped %d", layer, n, pc->step_rows);
-  if (int rc = reach_table(c, mapped_reach(pc))) return rc;
+  if (int rc = reach_table(c, pc->reach)) return rc;
   if (layer == 0) {
     MapArgs a = map_of(pc);
     a.n = n;
+    a.reach = reach_with(c, pc);
     a.ids = seq_ids;
     a.slots = pc->step_slots;
     a.positions = pc->step_positions;
@@ -510,7 +531,7 @@ int shainet_attn_forward_paged(shainet_attn_ctx *c, shainet_paged_cache *pc, int
   if (n_seqs < 1 || n_seqs > SHAINET_HIP_MAX_BATCH) return fail(SHAINET_HIP_ERR_ARGUMENT, "n_seqs must be in 1..%d", SHAINET_HIP_MAX_BATCH);
   if (int rc = refuse_recording(c, "shainet_attn_forward_paged")) return rc;
   if (int rc = refuse_unknown_lengths(pc, "shainet_attn_forward_paged")) return rc;
-  int ids[kMaxSeqs], start[kMaxSeqs], change[kMaxSeqs], longest = 0;
+  int ids[kMaxSeqs], start[kMaxSeqs], change[kMaxSeqs], longest = 0, furthest = 0;
   long long total = 0, pages = 0;
   for (int s = 0; s < n_seqs; ++s) {
     const int id = ids[s] = seq_ids ? seq_ids[s] : s, more = change[s] = new_tokens[s];
@@ -527,6 +548,7 @@ int shainet_attn_forward_paged(shainet_attn_ctx *c, shainet_paged_cache *pc, int
     total += more;
     if (total > 0x3fffffff / (c->H + 2 * c->KV)) return fail(SHAINET_HIP_ERR_ARGUMENT, "too many rows in one call");
     if (more > kRowsFromPages && start[s] + more > longest) longest = start[s] + more;
+    if (start[s] + more > furthest) furthest = start[s] + more;
   }
   if (layer == 0 && pages > pc->free_count)
     return fail(SHAINET_HIP_ERR_CAPACITY, "%lld pages wanted, %d free", pages, pc->free_count);
@@ -535,7 +557,10 @@ int shainet_attn_forward_paged(shainet_attn_ctx *c, shainet_paged_cache *pc, int
     return fail(SHAINET_HIP_ERR_ARGUMENT, "layer %d: other rows than layer 0 of this cache had last", layer);
   const int rows = (int)total;
   const size_t q_floats = (size_t)rows * c->H * c->hd, kv_floats = (size_t)rows * c->KV * c->hd, gathered = (size_t)c->KV * longest * c->hd;
-  int rc = reach_table(c, mapped_reach(pc));
+  const int reach = pc->reach;
+  extend_reach(pc, furthest);
+  int rc = reach_table(c, pc->reach);
+  if (rc) pc->reach = reach;
   if (!rc) rc = c->q_rot.reserve(q_floats);
   if (!rc && layer == 0) rc = pc->rows.reserve(3 * (size_t)rows);
   if (!rc && longest) rc = pc->gathered.reserve(2 * gathered);
@@ -573,7 +598,7 @@ int shainet_attn_forward_paged(shainet_attn_ctx *c, shainet_paged_cache *pc, int
       pc->last_ids.clear();
       rc = fail(SHAINET_HIP_ERR_ALLOC, "out of host memory");
     }
-    if (!rc) rc = map_listed(pc, ids, start, change, n_seqs, lists, rows);
+    if (!rc) rc = map_listed(pc, ids, start, change, n_seqs, reach_with(c, pc), lists, rows);
     if (rc) {
       if (mem == SHAINET_HIP_MEM_HOST) (void)hipStreamSynchronize(c->stream);
       return rc;
@@ -608,7 +633,7 @@ int shainet_attn_forward_paged(shainet_attn_ctx *c, shainet_paged_cache *pc, int
         start[s] += change[s];
         change[s] = -change[s];
       }
-      (void)map_listed(pc, ids, start, change, n_seqs, nullptr, 0);
+      (void)map_listed(pc, ids, start, change, n_seqs, 0, nullptr, 0);
       pc->last_ids.clear();
     }
     if (mem == SHAINET_HIP_MEM_HOST) (void)hipStreamSynchronize(c->stream);

@@ -150,7 +150,10 @@ __global__ __launch_bounds__(THREADS) void page_map_kernel(MapArgs a) {
   __shared__ unsigned named[kMaxPagedSeqs / 32];
   __shared__ int bad, last;
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6, each = EACH == 1 ? 1 : (a.n + THREADS - 1) / THREADS;
-  const int top = *a.n_free, epoch = *a.epoch;
+  const int2 words = *(const int2 *)a.n_free;
+  const int top = words.x;
+  int epoch = words.y;
+  int *rows_epoch = a.rows_epoch;
   const long long most = (long long)a.seq_pages << a.shift;
   int id[EACH], change[EACH], old_len[EACH], new_len[EACH];
 #pragma unroll
@@ -168,6 +171,7 @@ __global__ __launch_bounds__(THREADS) void page_map_kernel(MapArgs a) {
   int rows = 0, gone = 0, taken = 0;
   float rows_about = 0.0f;
   bool wrong = top < 0 || top > a.n_pages, full = false;
+  asm volatile("" : "+s"(epoch), "+s"(rows_epoch));  // (not fetched at the end, behind everything)
 #pragma unroll
   for (int u = 0; u < EACH; ++u) {
     const int s = id[u], d = change[u];
@@ -184,7 +188,7 @@ __global__ __launch_bounds__(THREADS) void page_map_kernel(MapArgs a) {
       wrong = true;
       continue;
     }
-    if (now > most || d > a.max_rows) {
+    if (now > most || d > a.max_rows || (d > 0 && now > a.reach)) {
       full = true;
       continue;
     }
@@ -265,12 +269,11 @@ __global__ __launch_bounds__(THREADS) void page_map_kernel(MapArgs a) {
     if (u < each && t * each + u < a.n && ok) a.lens[id[u]] = new_len[u];
   if (t == 0) {
     if (ok) {
-      *a.n_free = top + all[1] - all[2];
-      *a.epoch = epoch + 1;
+      *(int2 *)a.n_free = int2{top + all[1] - all[2], epoch + 1};
     } else {
       *(volatile int *)a.error = bad & 1 ? kMapBadEntry : kMapNoRoom;
     }
-    if (a.rows_epoch) *a.rows_epoch = ok ? epoch + 1 : epoch;
+    if (rows_epoch) *rows_epoch = ok ? epoch + 1 : epoch;
   }
 }
 
@@ -291,18 +294,18 @@ __global__ __launch_bounds__(1024) void page_report_kernel(MapArgs a, int *host,
       gone = 1;
   }
   gone = __syncthreads_or(gone);
-  if (threadIdx.x == 0 && gone) *a.epoch += 1;
+  if (threadIdx.x == 0 && gone) a.n_free[1] += 1;
   __syncthreads();
   for (int i = threadIdx.x; i < a.n_seqs + words; i += 1024) host[i] = i < a.n_seqs ? a.lens[i] : a.n_free[i - a.n_seqs];
 }
 
-__global__ __launch_bounds__(256) void page_reset_kernel(int *lens, int n_seqs, int *free_pages, int *n_free, int n_pages, int *epoch) {
+__global__ __launch_bounds__(256) void page_reset_kernel(int *lens, int n_seqs, int *free_pages, int *n_free, int n_pages) {
   const int i = blockIdx.x * 256 + threadIdx.x;
   if (i < n_seqs) lens[i] = 0;
   if (i < n_pages) free_pages[i] = n_pages - 1 - i;
   if (i == 0) {
     *n_free = n_pages;
-    *epoch += 1;
+    n_free[1] += 1;
   }
 }
 
@@ -332,10 +335,10 @@ hipError_t launch_page_report(const MapArgs &a, int *host, int words, hipStream_
   return hipGetLastError();
 }
 
-hipError_t launch_page_reset(int *lens, int n_seqs, int *free_pages, int *n_free, int n_pages, int *epoch, hipStream_t stream) {
+hipError_t launch_page_reset(int *lens, int n_seqs, int *free_pages, int *n_free, int n_pages, hipStream_t stream) {
   const int items = n_seqs > n_pages ? n_seqs : n_pages;
   hipLaunchKernelGGL(page_reset_kernel, dim3((unsigned)((items + 255) / 256)), dim3(256), 0, stream, lens, n_seqs, free_pages,
-                     n_free, n_pages, epoch);
+                     n_free, n_pages);
   return hipGetLastError();
 }
 
