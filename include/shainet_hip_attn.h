@@ -298,7 +298,8 @@ int shainet_attn_step_paged(shainet_attn_ctx *ctx, shainet_paged_cache *cache, i
                             const float *q, const float *k, const float *v, float *out);
 /* shainet_attn_forward over a cache in pages: any number of new rows for each of up to SHAINET_HIP_MAX_BATCH sequences (host
  * arrays seq_ids and new_tokens), planned on the host, which must know the lengths.  Sequences with more than a few new rows
- * have their pages gathered into one piece of float32 scratch (which grows on demand) first and run as any prompt does.  Layer 0
+ * have their pages gathered into one piece of float32 scratch (which grows on demand) first and run as any prompt does; keys of such a
+ * sequence in no page of the pool cannot be left out there, and the next call that waits returns SHAINET_HIP_ERR_ARGUMENT.  Layer 0
  * maps and counts the rows; calls for the layers behind it give the same seq_ids and new_tokens.  Not to be recorded: the lengths are part of
  * the plan.  SHAINET_HIP_ERR_CAPACITY, and nothing appended, when a sequence would outgrow its table or the pages do not
  * suffice. */

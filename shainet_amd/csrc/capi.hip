@@ -71,6 +71,10 @@ int check_error_word(int *w) {
     return fail(SHAINET_HIP_ERR_CAPACITY,
                 "a layer behind the first found rows behind the end of its context's cos/sin table (shainet_paged_cache_lengths_from_device "
                 "lets the next call extend it): they were neither placed nor attended");
+  if (what == kKeysOutside)
+    return fail(SHAINET_HIP_ERR_ARGUMENT,
+                "a forward call of more than a few rows for a sequence found keys in no page of the pool: its outputs for that sequence are "
+                "none (its rows are placed; truncate takes them back, and calls of up to 8 rows leave such keys out)");
   if (what == 2)
     return fail(SHAINET_HIP_ERR_CAPACITY,
                 "a decode step found a sequence at the capacity of its cache or at the end of the context's "

@@ -35,7 +35,7 @@ struct MapArgs {
   int *scratch;                // a word, zero, which a launch leaves so
   int *error;                  // device-writable: set to kMapNoRoom or kMapBadEntry where nothing was changed
 };
-constexpr int kMapNoRoom = 3, kMapBadEntry = 4, kRowsGone = 5, kRowsFar = 6;
+constexpr int kMapNoRoom = 3, kMapBadEntry = 4, kRowsGone = 5, kRowsFar = 6, kKeysOutside = 7;
 hipError_t launch_page_map(const MapArgs &a, hipStream_t stream);
 // every length 0, every page free, page 0 to be taken first
 hipError_t launch_page_reset(int *lens, int n_seqs, int *free_pages, int *n_free, int n_pages, hipStream_t stream);
@@ -71,7 +71,8 @@ struct PagedAttendArgs {
 size_t paged_attend_workspace(int hd);
 hipError_t launch_paged_attend(const PagedAttendArgs &a, const PagePool &p, hipStream_t stream);
 
-// The first n rows of a sequence, as floats, into [KV][cap][hd] arrays.
-hipError_t launch_page_gather(const PagePool &p, int seq, int pos0, int n, int cap, float *k, float *v, hipStream_t stream);
+// Rows pos0 .. pos0 + n - 1 of a sequence, as floats, into [KV][cap][hd] arrays.  A row in no page of the pool is zeros, and *error (if any)
+// kKeysOutside.
+hipError_t launch_page_gather(const PagePool &p, int seq, int pos0, int n, int cap, float *k, float *v, int *error, hipStream_t stream);
 
 }  // namespace shainet

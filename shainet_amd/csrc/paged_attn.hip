@@ -839,13 +839,14 @@ __device__ __forceinline__ long long page_row(const PagePool &p, const int *tabl
 }
 
 template <int DTYPE>
-__global__ __launch_bounds__(256) void page_gather_kernel(PagePool p, int seq, int pos0, int n, int cap, float *k, float *v) {
+__global__ __launch_bounds__(256) void page_gather_kernel(PagePool p, int seq, int pos0, int n, int cap, float *k, float *v, int *error) {
   const int per = p.hd >> 2;
   const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
   if (i >= (long long)n * p.KV * per) return;
   const int piece = (int)(i % per), t = (int)(i / per % n), c = (int)(i / per / n);
   const long long row = page_row(p, p.table + (long long)seq * p.seq_pages, pos0 + t, c);
   const long long to = ((long long)c * cap + t) * p.hd + 4 * piece;
+  if (row < 0 && error && c == 0 && piece == 0 && *(volatile int *)error == 0) *(volatile int *)error = kKeysOutside;  // (a map that failed before says why)
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     if (k) k[to + e] = row < 0 ? 0.0f : page_value<DTYPE>(p.k, row * p.hd + 4 * piece + e);
@@ -897,7 +898,7 @@ hipError_t launch_paged_attend(const PagedAttendArgs &a, const PagePool &p, hipS
   return p.dtype == kPageF32 ? launch_attend<kPageF32>(a, p, stream) : p.dtype == kPageBf16 ? launch_attend<kPageBf16>(a, p, stream) : launch_attend<kPageF16>(a, p, stream);
 }
 
-hipError_t launch_page_gather(const PagePool &p, int seq, int pos0, int n, int cap, float *k, float *v, hipStream_t stream) {
+hipError_t launch_page_gather(const PagePool &p, int seq, int pos0, int n, int cap, float *k, float *v, int *error, hipStream_t stream) {
   if (n < 1) return hipSuccess;
   if (seq < 0 || seq >= p.n_seqs || pos0 < 0 || (long long)pos0 + n > (long long)p.seq_pages << p.shift || n > cap)
     return hipErrorInvalidValue;
@@ -906,7 +907,7 @@ hipError_t launch_page_gather(const PagePool &p, int seq, int pos0, int n, int c
   const auto kernel = p.dtype == kPageF32    ? page_gather_kernel<kPageF32>
                       : p.dtype == kPageBf16 ? page_gather_kernel<kPageBf16>
                                              : page_gather_kernel<kPageF16>;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, stream, p, seq, pos0, n, cap, k, v);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, stream, p, seq, pos0, n, cap, k, v, error);
   return hipGetLastError();
 }
 

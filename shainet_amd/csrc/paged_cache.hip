@@ -458,7 +458,7 @@ int shainet_paged_cache_read(shainet_paged_cache *pc, int layer, int seq, int kv
   const size_t each = (size_t)pc->KV * n * pc->hd;
   if (int rc = pc->gathered.reserve(2 * each)) return rc;
   float *k = pc->gathered.p, *v = k + each;
-  const hipError_t e = launch_page_gather(pool_of(pc, layer), seq, pos0, n, n, k, v, pc->ctx->stream);
+  const hipError_t e = launch_page_gather(pool_of(pc, layer), seq, pos0, n, n, k, v, nullptr, pc->ctx->stream);
   if (e != hipSuccess) return hip_fail(e, "gather launch");
   HIP_TRY(hipStreamSynchronize(pc->ctx->stream));
   const size_t first = (size_t)kv_head * n * pc->hd, bytes = (size_t)n * pc->hd * sizeof(float);
@@ -620,7 +620,7 @@ int shainet_attn_forward_paged(shainet_attn_ctx *c, shainet_paged_cache *pc, int
     if (many) {
       const int cap = start[s] + change[s];
       float *gk = pc->gathered.p, *gv = gk + gathered;
-      const hipError_t e = launch_page_gather(pool_of(pc, layer), ids[s], 0, cap, cap, gk, gv, c->stream);
+      const hipError_t e = launch_page_gather(pool_of(pc, layer), ids[s], 0, cap, cap, gk, gv, pc->ctx->error, c->stream);
       rc = e == hipSuccess ? shainet_attn_run_rows(c, c->q_rot.p + at * q_dim, gk, gv, cap, start[s], change[s], dout + at * q_dim)
                            : hip_fail(e, "gather launch");
       done = at + change[s];

@@ -93,6 +93,33 @@ def test_rows_of_a_call_that_the_host_plans(hip, torch):  # noqa: F811
             far.check(layer, x, got, list(range(n, n + new)))
 
 
+@pytest.mark.parametrize("mode", ["device", "host"])
+@pytest.mark.parametrize("new", [9, 20])
+def test_prompts_on_keys_of_no_page(hip, torch, new, mode):  # noqa: F811
+    """More rows than are attended one by one: such keys would count as zeros there, and the call is reported; its rows can be taken back."""
+    far = Far(hip, torch, np.random.default_rng(5))
+    cache, ctx = far.cache, far.ctxs[0]
+    cache.lengths_from_device()
+    x = far.rows(new)
+    with pytest.raises(hip.ArgumentError, match="no page of the pool"):
+        if mode == "device":
+            ctx.forward_paged(cache, *x, [new], seq_ids=[0])
+            ctx.sync()
+        else:
+            ctx.forward_paged(cache, *(t.cpu().numpy() for t in x), [new], seq_ids=[0])
+    assert cache.len(0) == 2000 + new and cache.lens.tolist() == [2000 + new, 0]
+    cache.truncate(0, 2000)
+    ctx.sync()
+    assert cache.free_page_count() == 4
+    got = ctx.forward_paged(cache, *(t[:8].contiguous() for t in x), [8], seq_ids=[0])
+    ctx.sync()
+    far.check(0, [t[:8] for t in x], got, list(range(2000, 2008)))
+    # a sequence of pages of its own beside it
+    y = far.rows(new)
+    ctx.forward_paged(cache, *y, [new], seq_ids=[1])
+    ctx.sync()
+
+
 def test_a_layer_whose_table_of_angles_is_shorter(hip, torch):  # noqa: F811
     far = Far(hip, torch, np.random.default_rng(3), positions=(4000, 0))
     cache, zero = far.cache, _ints(torch, [0])
