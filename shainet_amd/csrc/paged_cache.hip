@@ -562,14 +562,17 @@ int shainet_attn_forward_paged(shainet_attn_ctx *c, shainet_paged_cache *pc, int
   int rc = reach_table(c, pc->reach);
   if (rc) pc->reach = reach;
   if (!rc) rc = c->q_rot.reserve(q_floats);
-  if (!rc && layer == 0) rc = pc->rows.reserve(3 * (size_t)rows);
   if (!rc && longest) rc = pc->gathered.reserve(2 * gathered);
   const float *dq = q, *dk = k, *dv = v;
   float *dout = out;
-  if (!rc && mem == SHAINET_HIP_MEM_HOST) {
+  if (!rc && mem == SHAINET_HIP_MEM_HOST)
     (void)((rc = c->in_q.reserve(q_floats)) || (rc = c->in_k.reserve(kv_floats)) || (rc = c->in_v.reserve(kv_floats)) ||
            (rc = c->out.reserve(q_floats)) || (rc = c->pin_in.reserve(q_floats + 2 * kv_floats)) || (rc = c->pin_out.reserve(q_floats)));
-    if (rc) return rc;
+  // (the last call's lists go when nothing else can be lacking any more: until then its other layers use them)
+  if (!rc && layer == 0) rc = pc->rows.reserve(3 * (size_t)rows);
+  if (rc) return rc;
+  if (layer == 0) forget_rows(pc);
+  if (mem == SHAINET_HIP_MEM_HOST) {
     float *pq = c->pin_in.p, *pk = pq + q_floats, *pv = pk + kv_floats;
     memcpy(pq, q, q_floats * sizeof(float));
     memcpy(pk, k, kv_floats * sizeof(float));
@@ -586,20 +589,19 @@ int shainet_attn_forward_paged(shainet_attn_ctx *c, shainet_paged_cache *pc, int
     dv = c->in_v.p;
     dout = c->out.p;
   }
-  if (rc) return rc;
   int *lists = (int *)pc->rows.p;
   const int *slots = lists, *positions = lists + rows;
   int *row_seqs = lists + 2 * (size_t)rows;
   if (layer == 0) {
     try {
-      pc->last_ids.assign(ids, ids + n_seqs);
       pc->last_new.assign(change, change + n_seqs);
+      pc->last_ids.assign(ids, ids + n_seqs);
     } catch (const std::bad_alloc &) {
-      pc->last_ids.clear();
       rc = fail(SHAINET_HIP_ERR_ALLOC, "out of host memory");
     }
     if (!rc) rc = map_listed(pc, ids, start, change, n_seqs, reach_with(c, pc), lists, rows);
     if (rc) {
+      forget_rows(pc);
       if (mem == SHAINET_HIP_MEM_HOST) (void)hipStreamSynchronize(c->stream);
       return rc;
     }
@@ -634,7 +636,7 @@ int shainet_attn_forward_paged(shainet_attn_ctx *c, shainet_paged_cache *pc, int
         change[s] = -change[s];
       }
       (void)map_listed(pc, ids, start, change, n_seqs, 0, nullptr, 0);
-      pc->last_ids.clear();
+      forget_rows(pc);
     }
     if (mem == SHAINET_HIP_MEM_HOST) (void)hipStreamSynchronize(c->stream);
     return rc;
@@ -642,7 +644,6 @@ int shainet_attn_forward_paged(shainet_attn_ctx *c, shainet_paged_cache *pc, int
   if (layer == 0) {
     for (int s = 0; s < n_seqs; ++s) pc->len[ids[s]] += change[s];
     pc->free_count -= (int)pages;
-    pc->step_rows = 0;
   }
   c->last_rows = rows;
   if (mem == SHAINET_HIP_MEM_HOST) {

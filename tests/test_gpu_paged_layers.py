@@ -206,3 +206,31 @@ def test_layers_of_a_step_against_the_definition(hip, torch, dtype):  # noqa: F8
                 want, off = attended(turned, k, v)
                 # (queries turned in float32 are off by 6 u of a pair's size at most, in every score, which `attended` allows hd + 4 of)
                 assert (np.abs(outs[layer][s] - want) <= 1.5 * off).all(), (turn, layer, s)
+
+
+def test_a_call_without_memory_leaves_the_rows_of_the_one_before(hip, torch):  # noqa: F811
+    """400 GB of gathered rows are not to be had: the call changes nothing, and the last one's other layers go on."""
+    rng = np.random.default_rng(6)
+    heads, hd = 2048, 8
+    ctx = hip.AttnContext(heads, heads, hd)
+    ctx.set_stream(torch.cuda.current_stream().cuda_stream)
+    cache = hip.PagedKVCache(ctx, 4, 1024, 2, 3100, layers=2)
+    cache.table[1].fill_(-1)  # (a long sequence whose pages were dropped)
+    cache.lens[1] = 3_000_000
+    cache.lengths_from_device()
+    x = _rows(torch, rng, 3, heads, heads, hd)
+    ctx.forward_paged(cache, *x, [3], seq_ids=[0])
+    ctx.sync()
+    with pytest.raises(hip.HipError, match="hipMalloc"):
+        ctx.forward_paged(cache, *_rows(torch, rng, 400, heads, heads, hd), [400], seq_ids=[1])
+    assert (cache.len(0), cache.len(1), cache.free_page_count()) == (3, 3_000_000, 3)
+    got = ctx.forward_paged(cache, *x, [3], seq_ids=[0], layer=1)
+    ctx.sync()
+    assert cache.lens.tolist() == [3, 3_000_000] and cache.n_free.item() == 3
+    v = x[2].view(3, heads, hd).to(torch.bfloat16)
+    page = cache.table[0, 0].item()
+    assert torch.equal(cache.pages(1)[1][page, :, :3], v.transpose(0, 1))
+    # (one key: its value, w v (1 / w) for a weight w near 1; the first product, the quotient and the second product are rounded by half
+    # a step, 2^-24, each)
+    want = v[0].float().flatten()
+    assert ((got[0] - want).abs() <= 3.01 * 2.0 ** -24 * want.abs()).all()
