@@ -222,12 +222,17 @@ int append(shainet_attn_ctx *c, shainet_paged_cache *pc, int layer, const PrepAr
   return e == hipSuccess ? SHAINET_HIP_OK : hip_fail(e, "append launch");
 }
 
-int attend(shainet_attn_ctx *c, shainet_paged_cache *pc, int layer, const int *row_seqs, const int *positions, int rows,
-           const float *q, long long q_stride, float *out, long long out_stride) {
-  // (tiles of 16 keys are counted in 32 bits, and those of a workgroup's span of all pairs)
+// Tiles of 16 keys are counted in 32 bits, and so are those of a workgroup's span of all pairs.
+int refuse_many_keys(const shainet_attn_ctx *c, const shainet_paged_cache *pc, int rows) {
   if (rows * reach_of(pc) >= 1LL << 34 || rows * reach_of(pc) * c->KV * ((c->g + 15) / 16) >= 1LL << 42)
     return fail(SHAINET_HIP_ERR_ARGUMENT, "%d rows of up to %lld keys in one call: their product must stay below 2^34, and times the kv heads below 2^42",
                 rows, reach_of(pc));
+  return SHAINET_HIP_OK;
+}
+
+int attend(shainet_attn_ctx *c, shainet_paged_cache *pc, int layer, const int *row_seqs, const int *positions, int rows,
+           const float *q, long long q_stride, float *out, long long out_stride) {
+  if (int rc = refuse_many_keys(c, pc, rows)) return rc;
   PagedAttendArgs a;
   a.q = q;
   a.out = out;
@@ -497,6 +502,7 @@ int shainet_attn_step_paged(shainet_attn_ctx *c, shainet_paged_cache *pc, int la
   if (n < 1 || n > pc->n_seqs) return fail(SHAINET_HIP_ERR_ARGUMENT, "n must be in 1..%d", pc->n_seqs);
   if (layer > 0 && n != pc->step_rows)
     return fail(SHAINET_HIP_ERR_ARGUMENT, "layer %d of a step of %d rows: layer 0 mapped %d", layer, n, pc->step_rows);
+  if (int rc = refuse_many_keys(c, pc, n)) return rc;  // (before a row is mapped)
   if (int rc = reach_table(c, pc->reach)) return rc;
   if (layer == 0) {
     MapArgs a = map_of(pc);

@@ -178,3 +178,24 @@ def test_recorded_steps_have_the_table_that_they_were_recorded_with(hip, torch):
                     ctx.sync()
                 assert (out == 5.0).all()
             assert cache.lens.tolist() == [n, 1]
+
+
+def test_a_step_of_more_keys_than_can_be_counted(hip, torch):  # noqa: F811
+    """Tables wide enough for 2^30 keys: a step of so many rows is refused before it maps one."""
+    ctx = hip.AttnContext(1024, 1024, 8)
+    ctx.set_stream(torch.cuda.current_stream().cuda_stream)
+    cache = hip.PagedKVCache(ctx, 20, 1024, 16, 2 ** 20 - 1)
+    x = [torch.ones((16, 1024 * 8), device="cuda") for _ in range(3)]
+    out = torch.full_like(x[0], 5.0)
+    for n in (16, 15, 5):
+        with pytest.raises(hip.ArgumentError, match="2\\^42"):
+            ctx.step_paged(cache, *(t[:n] for t in x), out[:n])
+    assert cache.len(0) == 0 and cache.free_page_count() == 20  # (the host still knows)
+    with pytest.raises(hip.ArgumentError, match="2\\^42"):
+        ctx.forward_paged(cache, *(t[:5] for t in x), [1] * 5)
+    cache.lengths_from_device()
+    assert [cache.len(s) for s in range(16)] == [0] * 16 and cache.free_page_count() == 20
+    ctx.step_paged(cache, *(t[:3] for t in x), out[:3])
+    cache.lengths_from_device()
+    assert [cache.len(s) for s in range(4)] == [1, 1, 1, 0] and (out[3:] == 5.0).all()
+    assert ((out[:3] - 1).abs() <= 3.01 * 2.0 ** -24).all()  # (one key: its value, by two products and a quotient, each rounded)
