@@ -275,7 +275,7 @@ int shainet_paged_cache_read(shainet_paged_cache *cache, int layer, int seq, int
 /* Bias, QK-norm and RoPE of `rows` rows of q, k and v (device pointers, rows at the given strides), as shainet_attn_forward
  * does them: rotated queries to q_rot [rows, num_heads*head_dim], K and V rows to slots[row], rotated by positions[row].
  * Rows whose slot is no slot of the cache or whose position is outside the cos/sin table (those of a map at -1) are left
- * alone, in q_rot too.  Slots are distinct.  Asynchronous on the context's stream. */
+ * alone, in q_rot too.  Slots are distinct.  q_rot may be q, if q's rows are dense; else it lies apart from q, k and v.  Asynchronous on the context's stream. */
 int shainet_attn_append_paged(shainet_attn_ctx *ctx, shainet_paged_cache *cache, int layer, const int *slots,
                               const int *positions, int rows, const float *q, long long q_stride, const float *k,
                               long long k_stride, const float *v, long long v_stride, float *q_rot);
@@ -284,7 +284,7 @@ int shainet_attn_append_paged(shainet_attn_ctx *ctx, shainet_paged_cache *cache,
  * row_seqs outside 0..n_seqs-1 leaves its output alone; one with positions < 0, or whose keys' pages are all outside the
  * pool, gets zeros; one that sees an infinite number or none gets outputs that are infinite or no numbers.  At most
  * SHAINET_HIP_MAX_PAGED_SEQS rows, and rows * seq_pages * page_rows below 2^34, times num_kv_heads (once for every 16 query
- * heads of each) below 2^42.  Rows of q_rot and out at the given strides; out may be q_rot.  Asynchronous on the context's stream.  Scores, softmax and sums are float32, keys and values the pages'
+ * heads of each) below 2^42.  Rows of q_rot and out at the given strides; out may be q_rot at the same stride, else their rows lie apart.  Asynchronous on the context's stream.  Scores, softmax and sums are float32, keys and values the pages'
  * numbers as they are.  Replays of recordings that use one cache must not overlap. */
 int shainet_attn_attend_paged(shainet_attn_ctx *ctx, shainet_paged_cache *cache, int layer, const int *row_seqs,
                               const int *positions, int rows, const float *q_rot, long long q_stride, float *out,

@@ -2,6 +2,7 @@
 // AttnContext over them (declared in include/shainet_hip_attn.h).
 #include <hip/hip_runtime.h>
 #include <stdarg.h>
+#include <stdint.h>
 #include <stdio.h>
 #include <string.h>
 
@@ -249,6 +250,19 @@ int attend(shainet_attn_ctx *c, shainet_paged_cache *pc, int layer, const int *r
   return e == hipSuccess ? SHAINET_HIP_OK : hip_fail(e, "attention launch");
 }
 
+// Whether writing a row of b can change a row of a that somebody still reads: rows of `width` floats at a distance each.  Where the rows are the
+// same ones, each is written by those that read it, behind that.
+bool in_the_way(const float *a, long long a_stride, long long a_width, const float *b, long long b_stride, long long b_width, int rows) {
+  const long long last_a = (rows - 1) * a_stride + a_width, last_b = (rows - 1) * b_stride + b_width;
+  const uintptr_t from_a = (uintptr_t)a, from_b = (uintptr_t)b;
+  if (from_a + last_a * sizeof(float) <= from_b || from_b + last_b * sizeof(float) <= from_a) return false;
+  if (rows == 1) return a != b || a_width != b_width;
+  if (a_stride != b_stride) return true;  // (some could still lie between each other)
+  if (a == b) return a_width != b_width;
+  const long long step = a_stride * (long long)sizeof(float), d = (long long)(from_b - from_a), behind = ((d % step) + step) % step;
+  return behind < a_width * (long long)sizeof(float) || step - behind < b_width * (long long)sizeof(float);
+}
+
 // New rows of a sequence up to this many read the pages themselves, one by one; for more the pages are gathered first, once for
 // all of them.  32 heads of 128 on 8 kv heads, us from pages | gathered: 8 rows on 500 keys of float32 14.5 | 21, of bfloat16 10.6 | 20; on
 // 16000 160 | 166 and 85 | 117; 12 rows on 16000 233 | 199 and 115 | 169.
@@ -480,6 +494,10 @@ int shainet_attn_append_paged(shainet_attn_ctx *c, shainet_paged_cache *pc, int 
   if (rows < 1 || rows > 0x3fffffff / (c->H + 2 * c->KV)) return fail(SHAINET_HIP_ERR_ARGUMENT, "rows must be in 1..%d", 0x3fffffff / (c->H + 2 * c->KV));
   if (q_stride < (long long)c->H * c->hd || k_stride < (long long)c->KV * c->hd || v_stride < (long long)c->KV * c->hd)
     return fail(SHAINET_HIP_ERR_ARGUMENT, "row strides must be at least the row widths %d and %d", c->H * c->hd, c->KV * c->hd);
+  const long long q_dim = (long long)c->H * c->hd, kv_dim = (long long)c->KV * c->hd;
+  if (in_the_way(q, q_stride, q_dim, q_rot, q_dim, q_dim, rows) || in_the_way(k, k_stride, kv_dim, q_rot, q_dim, q_dim, rows) ||
+      in_the_way(v, v_stride, kv_dim, q_rot, q_dim, q_dim, rows))
+    return fail(SHAINET_HIP_ERR_ARGUMENT, "q_rot must lie apart from q, k and v, or be q with rows as far apart");
   if (int rc = reach_table(c, reach_of(pc))) return rc;
   return append(c, pc, layer, prep_of(c, q, q_stride, k, k_stride, v, v_stride, q_rot), slots, positions, rows, nullptr, 0);
 }
@@ -492,6 +510,9 @@ int shainet_attn_attend_paged(shainet_attn_ctx *c, shainet_paged_cache *pc, int 
     return fail(SHAINET_HIP_ERR_ARGUMENT, "rows must be in 1..%d", SHAINET_HIP_MAX_PAGED_SEQS);
   if (q_stride < (long long)c->H * c->hd || out_stride < (long long)c->H * c->hd)
     return fail(SHAINET_HIP_ERR_ARGUMENT, "row strides must be at least the row width %d", c->H * c->hd);
+  const long long q_dim = (long long)c->H * c->hd;
+  if (in_the_way(q_rot, q_stride, q_dim, out, out_stride, q_dim, rows))
+    return fail(SHAINET_HIP_ERR_ARGUMENT, "out must lie apart from q_rot, or be q_rot with rows as far apart");
   return attend(c, pc, layer, row_seqs, positions, rows, q_rot, q_stride, out, out_stride);
 }
 
