@@ -224,7 +224,8 @@ int shainet_attn_decode_step(shainet_attn_ctx *ctx, shainet_kv_cache *cache, int
  * the same kv heads and head_dim, at most as many query heads, and the same stream (shainet_attn_set_stream).
  * Calls that rotate rows extend their context's cos/sin table the first time, to as many positions as a sequence can have rows
  * (append_paged: to seq_pages * page_rows, whatever the number of pages), up to 8 GiB of it; that cannot be recorded
- * (SHAINET_HIP_ERR_ARGUMENT then).  Sequences that a caller made longer than the pool (see shainet_paged_cache_arrays) have their
+ * (SHAINET_HIP_ERR_ARGUMENT then).  The host computes the table (tens of milliseconds for 131072 positions of 64 pairs).  The shorter tables before it,
+ * less than twice as much together, stay for recordings until the context is destroyed.  Sequences that a caller made longer than the pool (see shainet_paged_cache_arrays) have their
  * positions there once the host knows the lengths; maps of steps and forward calls find no room behind the end of the table, and
  * layers behind the first, whose contexts may have shorter ones, place no row there and leave its output alone (SHAINET_HIP_ERR_CAPACITY by
  * the next call that waits).  Otherwise calls allocate nothing unless they say so.  Calls are made

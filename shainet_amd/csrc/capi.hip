@@ -15,6 +15,7 @@
 #include "attn_kernels.hpp"
 #include "block_kernels.hpp"
 #include "paged.hpp"
+#include "rope_table.hpp"
 
 using namespace shainet;
 
@@ -178,9 +179,7 @@ int upload(float **dst, const float *src, size_t n) {
 // llama_block.cr:274-277 does, for pos in [0, positions); rope_fp64: of pos * inv_freq64[i] instead.
 int shainet::ensure_rope_table(shainet_attn_ctx *c, int positions) {
   if (positions <= c->rope_positions) return SHAINET_HIP_OK;
-  int want = c->rope_positions ? c->rope_positions : 1024;
-  while (want < positions) want *= 2;
-  const int half = (int)c->inv_freq.size();
+  const int half = (int)c->inv_freq.size(), want = table_positions(c->rope_positions, positions, half * (int)sizeof(float2));
   if (half == 0) {
     c->rope_positions = want;
     return SHAINET_HIP_OK;
@@ -209,7 +208,8 @@ int shainet::ensure_rope_table(shainet_attn_ctx *c, int positions) {
     (void)hipFree(np);
     return hip_fail(e, "hipMemcpy(rope table)");
   }
-  // kernels already queued and recorded calls still read the old table; together the old ones are no larger than the new one
+  // kernels already queued and recorded calls still read the old table; each is half of the next at most but for
+  // the last, so together the old ones are less than twice the new one
   if (c->d_rope) c->old_rope.push_back(c->d_rope);
   c->d_rope = np;
   c->rope_positions = want;

@@ -14,6 +14,7 @@
 #include "attn_kernels.hpp"
 #include "llama_internal.hpp"
 #include "paged.hpp"
+#include "rope_table.hpp"
 
 using namespace shainet;
 
@@ -171,14 +172,11 @@ int map_listed(shainet_paged_cache *pc, const int *ids, const int *was, const in
   return e == hipSuccess ? SHAINET_HIP_OK : hip_fail(e, "map launch");
 }
 
-constexpr long long kMostTableBytes = 8LL << 30;
-long long most_positions(const shainet_attn_ctx *c) { return kMostTableBytes / ((long long)c->hd * 4); }
-
 // Sequences that hold pages of the pool only, each its own, are no longer than the pool; of those that a caller made longer (entries of
 // no page, pages shared) the host knows once it is told their lengths.
 void extend_reach(shainet_paged_cache *pc, long long rows) {
   if (rows <= pc->reach) return;
-  const long long most = most_positions(pc->ctx), more = 2 * rows < most ? 2 * rows : rows < most ? most : rows;
+  const long long most = most_table_positions(pc->hd * 4), more = 2 * rows < most ? 2 * rows : rows < most ? most : rows;
   pc->reach = (int)(more < reach_of(pc) ? more : reach_of(pc));
 }
 
@@ -188,7 +186,7 @@ int reach_table(shainet_attn_ctx *c, long long reach) {
   if (refuse_recording(c, ""))
     return fail(SHAINET_HIP_ERR_ARGUMENT, "the context's cos/sin table must be extended to %lld positions, which cannot be recorded: create the context "
                 "with that many, or place rows once before recording", reach);
-  if (reach > most_positions(c))
+  if (reach > most_table_positions(c->hd * 4))
     return fail(SHAINET_HIP_ERR_ALLOC, "a cos/sin table of %lld positions would take more than 8 GiB: the cache's table is that wide", reach);
   return ensure_rope_table(c, (int)reach);
 }
