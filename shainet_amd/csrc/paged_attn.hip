@@ -88,7 +88,7 @@ constexpr int kLongPair = 40;
 // ... and what the kernel makes of it.
 template <int DTYPE, int HD>
 struct Tile : PageTile<DTYPE, HD> {
-  static constexpr int PARTS = DTYPE == kPageF32 ? 1 : DTYPE == kPageBf16 ? 3 : 2;  // of a float operand
+  static constexpr int PARTS = DTYPE == kPageF32 ? 1 : 3;  // of a float operand
   static constexpr int WAVES = 4;                          // of a workgroup
   static constexpr int LONG = HD == 64 ? 160 : 40;         // tiles of a span that one workgroup on a compute unit reads faster than two
   // Tiles of a pair that is not worth being cut: one sequence of 100 keys (7 tiles of float32) 6.7 us | cut 8.4.
@@ -204,7 +204,8 @@ struct Wave {
 #pragma unroll
       for (int w = 0; w < T::PER / 4; ++w) raw.x[i][w] = query(rows, cols, first + i * step, w);
   }
-  // float16 parts hold 22 bits of a number between two of them, down to 2^-24: the largest of a row is brought to 2^14 .. 2^15
+  // Three float16 parts of 11 bits hold all 24 of a float, but none below 2^-24: the largest of a row is brought to 2^14 .. 2^15, so that
+  // numbers down to 2^-15 of it are exact and smaller ones, whose products vanish beside its, good to 2^-40 of it.
   __device__ __forceinline__ static float larger(float most, f32x4 x) {
     return fmaxf(most, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))));
   }
@@ -227,7 +228,7 @@ struct Wave {
       float y[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) y[e] = ldexpf(x[e >> 2][e & 3], down);
-      split_f16(y, part[0], part[1]);
+      split_f16(y, part);
     }
 #pragma unroll
     for (int i = 0; i < T::PARTS; ++i) to[(i * T::CHUNKS + u) * 64 + lane] = part[i];
@@ -255,12 +256,17 @@ struct Wave {
       put_query(to, x, u);
     }
   }
-  __device__ __forceinline__ static void split_f16(const float (&y)[8], u32x4 &high, u32x4 &low) {
+  __device__ __forceinline__ static void split_f16(const float (&y)[8], u32x4 (&part)[T::PARTS]) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const f16x2 h = f16x2{(_Float16)y[2 * e], (_Float16)y[2 * e + 1]};
-      high[e] = __builtin_bit_cast(unsigned, h);
-      low[e] = __builtin_bit_cast(unsigned, f16x2{(_Float16)(y[2 * e] - (float)h.x), (_Float16)(y[2 * e + 1] - (float)h.y)});
+      float a = y[2 * e], b = y[2 * e + 1];
+#pragma unroll
+      for (int i = 0; i < T::PARTS; ++i) {
+        const f16x2 h = f16x2{(_Float16)a, (_Float16)b};
+        part[i][e] = __builtin_bit_cast(unsigned, h);
+        a -= (float)h.x;
+        b -= (float)h.y;
+      }
     }
   }
   __device__ __forceinline__ static f32x4 mfma16(u32x4 a, u32x4 b, f32x4 x) {
@@ -346,7 +352,8 @@ struct Wave {
 #pragma unroll
         for (int e = 0; e < T::VEC; ++e) acc[u][e] *= fade;
     }
-    // (float16 parts of a weight: lifted by 2^15, as the queries are; the sum is lifted with them)
+    // (float16 parts of a weight: lifted by 2^15, as the queries are; the sum is lifted with them.  A weight of 2^-16 of the largest and less is
+    // good to 2^-40 of that one, which beside it no float32 sum keeps.)
     const float from = top == -INFINITY ? 0.0f : DTYPE == kPageF16 ? top - 15.0f : top;
     float w[KEYS_EACH];
 #pragma unroll
@@ -369,7 +376,7 @@ struct Wave {
       if constexpr (DTYPE == kPageBf16)
         split_octet(f32x4{w[0], w[1], w[2], w[3]}, f32x4{w[4], w[5], w[6], w[7]}, weights[0], weights[1], weights[2]);
       else
-        split_f16(w, weights[0], weights[1]);
+        split_f16(w, weights);
 #pragma unroll
       for (int u = 0; u < T::PIECES; ++u)
 #pragma unroll
