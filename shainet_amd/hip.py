@@ -713,7 +713,7 @@ class PagedKVCache:
             pool = (self.n_pages, self.ctx.num_kv_heads, self.page_rows, self.ctx.head_dim)
             shape = (pool, pool, (self.n_seqs, self.seq_pages), (self.n_seqs,), (self.n_pages,), (1,))[which]
             kind = ("<i4" if which > 1 else {"f32": "<f4", "bf16": "<i2", "f16": "<f2"}[self.dtype])
-            t = torch.as_tensor(_DeviceArray(self._handle, at[which].value, shape, kind), device="cuda")
+            t = torch.as_tensor(_DeviceArray(self._handle, at[which].value, shape, kind), device="cuda:%d" % self._device)
             self._views[which, layer] = t.view(torch.bfloat16) if which < 2 and self.dtype == "bf16" else t
         return self._views[which, layer]
 
