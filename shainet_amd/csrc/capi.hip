@@ -72,6 +72,10 @@ int check_error_word(int *w) {
     return fail(SHAINET_HIP_ERR_CAPACITY,
                 "a layer behind the first found rows behind the end of its context's cos/sin table (shainet_paged_cache_lengths_from_device "
                 "lets the next call extend it): they were neither placed nor attended");
+  if (what == kRowsOutside)
+    return fail(SHAINET_HIP_ERR_ARGUMENT,
+                "new rows were to go to a page that the pool does not have (a table entry or a free page that the caller wrote): they were neither "
+                "placed nor attended");
   if (what == kKeysOutside)
     return fail(SHAINET_HIP_ERR_ARGUMENT,
                 "a forward call of more than a few rows for a sequence found keys in no page of the pool: its outputs for that sequence are "

@@ -35,7 +35,7 @@ struct MapArgs {
   int *scratch;                // a word, zero, which a launch leaves so
   int *error;                  // device-writable: set to kMapNoRoom or kMapBadEntry where nothing was changed
 };
-constexpr int kMapNoRoom = 3, kMapBadEntry = 4, kRowsGone = 5, kRowsFar = 6, kKeysOutside = 7;
+constexpr int kMapNoRoom = 3, kMapBadEntry = 4, kRowsGone = 5, kRowsFar = 6, kKeysOutside = 7, kRowsOutside = 8;
 hipError_t launch_page_map(const MapArgs &a, hipStream_t stream);
 // every length 0, every page free, page 0 to be taken first
 hipError_t launch_page_reset(int *lens, int n_seqs, int *free_pages, int *n_free, int n_pages, hipStream_t stream);
@@ -46,10 +46,10 @@ hipError_t launch_page_report(const MapArgs &a, int *host, int words, hipStream_
 
 // Lists that a map for an earlier layer wrote: where lengths, tables or pages were changed since, the rows are nobody's or
 // another's.  Then none is placed, their row_seqs become -1 (so that attention leaves them alone) and *error kRowsGone; one at a position
-// that this layer's cos/sin table does not have goes the same way, with kRowsFar.
+// that this layer's cos/sin table does not have goes the same way, with kRowsFar, and one whose page is none of the pool with kRowsOutside.
 struct MappedRows {
   const int *epoch, *rows_epoch;  // (the same word: never)
-  int *row_seqs, *error;          // row_seqs null: lists of the caller's, or of the map just before
+  int *row_seqs, *error;          // row_seqs null: lists of the caller's
 };
 
 // bias -> QK-norm -> RoPE of `rows` rows, whose K and V parts go to slots[row] (page << shift | row in the page);

@@ -34,10 +34,12 @@ __device__ __forceinline__ PagedRow locate(const PrepArgs &a, const PagePool &p,
   const int slot = slots[token], hd = p.hd;
   const bool gone = *mapped.epoch != *mapped.rows_epoch;  // (asked for with the slot: no trip of its own)
   rr.pos = positions[token];
-  rr.valid = !gone && r < H + 2 * p.KV && (unsigned)slot < (unsigned)p.n_pages << p.shift && (unsigned)rr.pos < (unsigned)rope_positions;
-  if (mapped.row_seqs && r == 0 && (gone || rr.pos >= rope_positions)) {
+  const bool outside = (unsigned)slot >= (unsigned)p.n_pages << p.shift;
+  rr.valid = !gone && r < H + 2 * p.KV && !outside && (unsigned)rr.pos < (unsigned)rope_positions;
+  // (rows of a map that could not be made have positions -1, too)
+  if (mapped.row_seqs && r == 0 && rr.pos >= 0 && (gone || outside || rr.pos >= rope_positions)) {
     mapped.row_seqs[token] = -1;
-    *(volatile int *)mapped.error = gone ? kRowsGone : kRowsFar;
+    *(volatile int *)mapped.error = gone ? kRowsGone : outside ? kRowsOutside : kRowsFar;
   }
   rr.rotate = true;
   rr.dtype = kPageF32;

@@ -212,11 +212,11 @@ PrepArgs prep_of(const shainet_attn_ctx *c, const float *q, long long q_stride, 
   return pa;
 }
 
-// row_seqs: of rows that a map for layer 0 made, whose count is the word `of_map`; null: the caller's own lists, or just mapped
+// row_seqs: of rows that a map for layer 0 made, whose count is the word `of_map`; null: the caller's own lists
 int append(shainet_attn_ctx *c, shainet_paged_cache *pc, int layer, const PrepArgs &pa, const int *slots, const int *positions,
            int rows, int *row_seqs, int of_map) {
   const int *epoch = pc->n_free + kEpoch;
-  const MappedRows mapped = {epoch, row_seqs ? pc->n_free + of_map : epoch, row_seqs, pc->ctx->error};
+  const MappedRows mapped = {epoch, row_seqs && layer ? pc->n_free + of_map : epoch, row_seqs, pc->ctx->error};
   const hipError_t e = launch_paged_append(pa, pool_of(pc, layer), c->H, slots, positions, c->rope_positions, rows, mapped, c->stream);
   return e == hipSuccess ? SHAINET_HIP_OK : hip_fail(e, "append launch");
 }
@@ -542,7 +542,7 @@ int shainet_attn_step_paged(shainet_attn_ctx *c, shainet_paged_cache *pc, int la
   const long long q_dim = (long long)c->H * c->hd, kv_dim = (long long)c->KV * c->hd;
   float *q_rot = pc->step_q.p;
   if (int rc = append(c, pc, layer, prep_of(c, q, q_dim, k, kv_dim, v, kv_dim, q_rot), pc->step_slots, pc->step_positions, n,
-                      layer ? pc->step_seqs : nullptr, kStepEpoch))
+                      pc->step_seqs, kStepEpoch))
     return rc;
   return attend(c, pc, layer, pc->step_seqs, pc->step_positions, n, q_rot, q_dim, out, q_dim);
 }
@@ -633,7 +633,7 @@ int shainet_attn_forward_paged(shainet_attn_ctx *c, shainet_paged_cache *pc, int
   }
   const long long q_dim = (long long)c->H * c->hd, kv_dim = (long long)c->KV * c->hd;
   rc = append(c, pc, layer, prep_of(c, dq, q_dim, dk, kv_dim, dv, kv_dim, c->q_rot.p), slots, positions, rows,
-              layer ? row_seqs : nullptr, kForwardEpoch);
+              row_seqs, kForwardEpoch);
   // entries of a few rows each go together, from row `done` on; one of many by itself
   int at = 0, done = 0;
   for (int s = 0; s <= n_seqs && !rc; ++s) {

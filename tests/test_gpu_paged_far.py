@@ -199,3 +199,26 @@ def test_a_step_of_more_keys_than_can_be_counted(hip, torch):  # noqa: F811
     cache.lengths_from_device()
     assert [cache.len(s) for s in range(4)] == [1, 1, 1, 0] and (out[3:] == 5.0).all()
     assert ((out[:3] - 1).abs() <= 3.01 * 2.0 ** -24).all()  # (one key: its value, by two products and a quotient, each rounded)
+
+
+@pytest.mark.parametrize("where", ["free pages", "table"])
+def test_rows_that_have_no_page(hip, torch, where):  # noqa: F811
+    """A free page, or the entry of a sequence's last page, that the pool does not have: the row is left alone and reported, others are not."""
+    rng = np.random.default_rng(6)
+    far = Far(hip, torch, rng, positions=(4000, 4000))
+    cache, ctx = far.cache, far.ctxs[0]
+    if where == "table":  # sequence 0 goes on within its last page
+        cache.lens[0] = 1999
+        cache.table[0, 249] = 77
+    else:  # sequence 0 takes the first page
+        cache.free_pages[3] = -3
+    cache.lengths_from_device()
+    for layer in range(2):
+        x, out = far.rows(2), torch.full((2, H * HD), 5.0, device="cuda")
+        far.ctxs[layer].step_paged(cache, *x, out, layer=layer)
+        with pytest.raises(hip.ArgumentError, match="the pool does not have"):
+            ctx.sync()
+        assert (out[0] == 5.0).all()
+        # (one key: its value, by two products and a quotient, each rounded)
+        v = x[2][1].view(KV, 1, HD).expand(KV, H // KV, HD).reshape(-1)
+        assert ((out[1] - v).abs() <= 3.01 * 2.0 ** -24 * v.abs()).all()

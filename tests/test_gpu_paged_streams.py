@@ -84,3 +84,38 @@ def test_outputs_are_there_for_the_current_stream(hip, torch, name):  # noqa: F8
     got = side.call(name) + 0.0  # (no wait in between)
     torch.cuda.synchronize()
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_a_context_on_the_default_stream(hip, torch, name):  # noqa: F811
+    want = Side(hip, torch, torch.cuda.current_stream()).call(name)
+    side = Side(hip, torch, torch.cuda.default_stream())
+    torch.cuda.synchronize()
+    with torch.cuda.stream(torch.cuda.Stream()):
+        torch.cuda._sleep(LONG)
+        got = side.call(name) + 0.0
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("name", ["append", "attend"])
+def test_outputs_made_while_the_current_stream_is_recorded(hip, torch, name):  # noqa: F811
+    """The context's stream takes part in the recording by the waits, and leaves it by them."""
+    here, other = torch.cuda.Stream(), torch.cuda.Stream()
+    side = Side(hip, torch, other)
+    want = side.call(name)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=here):
+        got = side.call(name)
+        twice = got + got
+    for turn in range(4):
+        got.fill_(float("nan"))
+        twice.fill_(float("nan"))
+        torch.cuda.synchronize()
+        with torch.cuda.stream(here):
+            graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want) and torch.equal(twice, want + want), turn
+        side.x[1].add_(0.0)
+    del graph
