@@ -233,7 +233,9 @@ hipError_t launch_paged_append(const PrepArgs &a, const PagePool &p, int H, cons
   // squares side by side.  us a call, 48 head rows of 128 a token: without QK-norm 700 tokens 9.3 | 6.7 by four pairs, 170 as good; with
   // it 85 tokens 7.0 | 8.1 by LDS, 170 10.7 | 8.8, 1400 60 | 28.
   constexpr int kFewRows = 6144;
-  if (vec && n_rows >= kFewRows) {
+  // Heads over 128, of which a wavefront has no pair a lane: without QK-norm four pairs a lane, 1 to 180 rows of 24 heads of 256 2.5 to 3.5 us |
+  // by LDS 9.5 to 11.1; with it by LDS, whatever the rows.
+  if (vec && (n_rows >= kFewRows || p.hd > 128)) {
     const long long n_items = n_rows * (p.hd >> 3), blocks = (n_items + 255) / 256;
     if (blocks > 0x7fffffffLL) return hipErrorInvalidValue;
     hipLaunchKernelGGL(paged_rows_vec_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, a, p, H, slots, positions,
