@@ -222,14 +222,17 @@ int shainet_attn_decode_step(shainet_attn_ctx *ctx, shainet_kv_cache *cache, int
  * n_pages * page_rows, n_seqs * seq_pages below 2^31, seq_pages * page_rows below 2^30.  The context gives the head
  * geometry and the stream and must outlive the cache; contexts of other layers may use the cache too, with
  * the same kv heads and head_dim, at most as many query heads, and the same stream (shainet_attn_set_stream).
- * Calls that rotate rows extend their context's cos/sin table the first time, to as many positions as a sequence can have rows
- * (append_paged: to seq_pages * page_rows, whatever the number of pages), up to 8 GiB of it; that cannot be recorded
- * (SHAINET_HIP_ERR_ARGUMENT then).  The host computes the table (tens of milliseconds for 131072 positions of 64 pairs).  The shorter tables before it,
- * less than twice as much together, stay for recordings until the context is destroyed.  Sequences that a caller made longer than the pool (see shainet_paged_cache_arrays) have their
- * positions there once the host knows the lengths; maps of steps and forward calls find no room behind the end of the table, and
- * layers behind the first, whose contexts may have shorter ones, place no row there and leave its output alone (SHAINET_HIP_ERR_CAPACITY by
- * the next call that waits).  Otherwise calls allocate nothing unless they say so.  Calls are made
- * with the device current that was current at creation.  One caller at a time per cache. */
+ * Calls that rotate rows extend their context's cos/sin table the first time, to as many positions as a sequence can
+ * have rows (append_paged: to seq_pages * page_rows, whatever the number of pages), up to 8 GiB of it; that cannot be
+ * recorded (SHAINET_HIP_ERR_ARGUMENT then).  The host computes the table (tens of milliseconds for 131072 positions
+ * of 64 pairs).  The shorter tables before it, less than twice as much together, stay for recordings until the
+ * context is destroyed.  Sequences that a caller made longer than the pool (see shainet_paged_cache_arrays) have
+ * their positions there once the host knows the lengths; maps of steps and forward calls find no room behind the end
+ * of the table, and layers behind the first, whose contexts may have shorter ones, place no row there and leave its
+ * output alone.  Otherwise calls allocate nothing unless they say so.  What the device finds wrong with a call is
+ * returned by the next call that waits: shainet_attn_sync of the context that the cache was made with,
+ * shainet_paged_cache_lengths_from_device, or a forward call in host memory.  Calls are made with the device current
+ * that was current at creation.  One caller at a time per cache. */
 #define SHAINET_HIP_PAGE_F32 0
 #define SHAINET_HIP_PAGE_BF16 1
 #define SHAINET_HIP_PAGE_F16 2
@@ -241,7 +244,7 @@ int shainet_paged_cache_destroy(shainet_paged_cache *cache);
 /* Device addresses of the arrays above (K and V of one layer); any of the outputs may be null.  A caller that writes to
  * them itself (pages that sequences share, a table of its own scheduler) keeps that ordered with the context's stream and
  * calls shainet_paged_cache_lengths_from_device afterwards.  Kernels look at no page outside the pool, whatever the table says:
- * keys whose page is none of the n_pages take no part. */
+ * keys whose page is none of the n_pages take no part (but see shainet_attn_forward_paged). */
 int shainet_paged_cache_arrays(shainet_paged_cache *cache, int layer, void **k, void **v, int **table, int **lens,
                                int **free_pages, int **n_free);
 
@@ -252,8 +255,8 @@ int shainet_paged_cache_arrays(shainet_paged_cache *cache, int layer, void **k, 
  * Asynchronous on the context's stream, depends on nothing but its arguments: can be recorded and replayed, as append_paged,
  * attend_paged and step_paged can; the other calls are refused while the stream is recorded.  All or nothing: a sequence
  * out of range or named twice, a length below 0, or too few pages, too narrow a table or too many rows for the lists leave
- * lengths, table and stack as they were and all three lists at -1; the next shainet_attn_sync or
- * shainet_paged_cache_lengths_from_device then returns SHAINET_HIP_ERR_ARGUMENT or SHAINET_HIP_ERR_CAPACITY. */
+ * lengths, table and stack as they were and all three lists at -1; the next call that waits then returns SHAINET_HIP_ERR_ARGUMENT
+ * or SHAINET_HIP_ERR_CAPACITY. */
 int shainet_paged_cache_map_rows(shainet_paged_cache *cache, const int *seq_ids, const int *delta, int n, int *slots,
                                  int *positions, int *row_seqs, int max_rows);
 /* After calls that change lengths on the device (map_rows, step_paged) the host's copy is stale and shainet_attn_forward_paged,
@@ -290,11 +293,13 @@ int shainet_attn_append_paged(shainet_attn_ctx *ctx, shainet_paged_cache *cache,
 int shainet_attn_attend_paged(shainet_attn_ctx *ctx, shainet_paged_cache *cache, int layer, const int *row_seqs,
                               const int *positions, int rows, const float *q_rot, long long q_stride, float *out,
                               long long out_stride);
-/* A decode step: one new row for each of n sequences (seq_ids: device array, null: sequences 0..n-1); map, append and attend
- * with lists of the cache's own.  q [n, num_heads*head_dim], k, v [n, num_kv_heads*head_dim], out like q, device pointers.
- * Layer 0 maps the rows; calls for the layers behind it use that map (refused once lengths were changed otherwise; where the host
- * has not seen that, a replay for instance, they place nothing, leave `out` alone, and the next call that waits returns
- * SHAINET_HIP_ERR_ARGUMENT).  Can be recorded and replayed.  A step that found no room leaves `out` alone (see map_rows). */
+/* A decode step: one new row for each of n sequences (seq_ids: device array, null: sequences 0..n-1); map, append and
+ * attend with lists of the cache's own.  q [n, num_heads*head_dim], k, v [n, num_kv_heads*head_dim], out like q,
+ * device pointers. Layer 0 maps the rows; calls for the layers behind it use that map (refused once lengths were
+ * changed otherwise; where the host has not seen that, a replay for instance, they place nothing, leave `out` alone,
+ * and the next call that waits returns SHAINET_HIP_ERR_ARGUMENT).  Can be recorded and replayed.  A step that found
+ * no room leaves `out` alone (see map_rows), and one row that was to go to a page that the pool does not have leaves
+ * its part alone (SHAINET_HIP_ERR_ARGUMENT). */
 int shainet_attn_step_paged(shainet_attn_ctx *ctx, shainet_paged_cache *cache, int layer, const int *seq_ids, int n,
                             const float *q, const float *k, const float *v, float *out);
 /* shainet_attn_forward over a cache in pages: any number of new rows for each of up to SHAINET_HIP_MAX_BATCH sequences (host

@@ -881,7 +881,7 @@ hipError_t launch_attend(const PagedAttendArgs &a, const PagePool &p, hipStream_
 // Where there are more pairs than compute units two hide each other's beginnings and ends: 64 sequences of 100 to 300 keys
 // (512 pairs, float32) two 25 us | one 33, 39 of up to 5000 (312 pairs of heads of 64, tiles of half the bytes) 38 | 46.  How long their
 // spans are is known on the device only, where half of the workgroups leave if they are long: 64 sequences of 8192 to 32768 keys
-// (bfloat16) 763 us | two 780, 77 of up to 5000 (heads of 96, float16) 66 | 68.5, 100 of 1000 to 3000 (bfloat16) 132 | 137.  Where
+// (bfloat16) 763 us | two 780, 77 of up to 5000 (heads of 96, float16) 63 | 65.5, 100 of 1000 to 3000 (bfloat16) 132 | 137.  Where
 // pairs are short two are better whatever the spans: 128 of 1000 (32 tiles of bfloat16) 86 us | one 89, 700 of 100 to 700 228 | 257.
 template <int DTYPE, int HD>
 hipError_t launch_attend(const PagedAttendArgs &a, const PagePool &p, hipStream_t stream) {
