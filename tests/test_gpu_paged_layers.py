@@ -234,3 +234,34 @@ def test_a_call_without_memory_leaves_the_rows_of_the_one_before(hip, torch):  #
     # a step, 2^-24, each)
     want = v[0].float().flatten()
     assert ((got[0] - want).abs() <= 3.01 * 2.0 ** -24 * want.abs()).all()
+
+
+@pytest.mark.parametrize("rows", [8192, 8193, 70000])
+@pytest.mark.parametrize("where", [None, "first", "last", "middle"])
+def test_a_caller_that_writes_to_the_table_of_prompts(hip, torch, rows, where):  # noqa: F811
+    """Rows enough for a look by many workgroups: a page of one of two sequences is replaced, or none."""
+    ctx = hip.AttnContext(1, 1, 8)
+    ctx.set_stream(torch.cuda.current_stream().cuda_stream)
+    some = rows // 3
+    cache = hip.PagedKVCache(ctx, rows // 16 + 4, 16, 2, rows // 16 + 2, layers=2)
+    x = [torch.ones((rows, 8), device="cuda") for _ in range(3)]
+    forward = lambda layer: ctx.forward_paged(cache, *x, [some, rows - some], layer=layer)  # noqa: E731
+    forward(0)
+    if where == "first":
+        cache.table[0, 0] = cache.n_pages - 1
+    elif where == "last":
+        cache.table[1, (rows - some - 1) // 16] = cache.n_pages - 1
+    elif where == "middle":
+        cache.table[1, rows // 64] = cache.n_pages - 1
+    cache.lengths_from_device()
+    if where:
+        before = [t.clone() for t in cache.pages(1)]
+        with pytest.raises(hip.ArgumentError, match="layer 0"):
+            forward(1)
+        assert all(torch.equal(a, b) for a, b in zip(before, cache.pages(1)))
+    else:
+        out = forward(1)
+        ctx.sync()
+        # (values of 1: the outputs' numerator and the weights' sum are sums of as many numbers, each off by rows half steps at most)
+        assert ((out - 1).abs() <= (2 * rows + 40) * 2.0 ** -24).all()
+        assert (cache.pages(1)[1][cache.table[1, 0], :, :16] == 1).all()
