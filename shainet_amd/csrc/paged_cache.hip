@@ -251,14 +251,20 @@ int attend(shainet_attn_ctx *c, shainet_paged_cache *pc, int layer, const int *r
 // Whether writing a row of b can change a row of a that somebody still reads: rows of `width` floats at a distance each.  Where the rows are the
 // same ones, each is written by those that read it, behind that.
 bool in_the_way(const float *a, long long a_stride, long long a_width, const float *b, long long b_stride, long long b_width, int rows) {
-  const long long last_a = (rows - 1) * a_stride + a_width, last_b = (rows - 1) * b_stride + b_width;
-  const uintptr_t from_a = (uintptr_t)a, from_b = (uintptr_t)b;
-  if (from_a + last_a * sizeof(float) <= from_b || from_b + last_b * sizeof(float) <= from_a) return false;
-  if (rows == 1) return a != b || a_width != b_width;
-  if (a_stride != b_stride) return true;  // (some could still lie between each other)
-  if (a == b) return a_width != b_width;
-  const long long step = a_stride * (long long)sizeof(float), d = (long long)(from_b - from_a), behind = ((d % step) + step) % step;
-  return behind < a_width * (long long)sizeof(float) || step - behind < b_width * (long long)sizeof(float);
+  const long long word = sizeof(float), step_a = a_stride * word, step_b = b_stride * word, bytes_a = a_width * word, bytes_b = b_width * word;
+  const long long d = (long long)((uintptr_t)b - (uintptr_t)a);
+  if ((rows - 1) * step_a + bytes_a <= d || (rows - 1) * step_b + bytes_b <= -d) return false;
+  if (rows == 1 || (d == 0 && step_a == step_b)) return d != 0 || bytes_a != bytes_b;
+  if (step_a == step_b) {
+    const long long behind = ((d % step_a) + step_a) % step_a;
+    return behind < bytes_a || step_a - behind < bytes_b;
+  }
+  for (long long i = 0, j = 0; i < rows; ++i) {  // (the first row of b that ends behind where row i of a begins, and those that begin before its end)
+    while (j < rows && d + j * step_b + bytes_b <= i * step_a) ++j;
+    for (long long k = j; k < rows && d + k * step_b < i * step_a + bytes_a; ++k)
+      if (k != i || d + k * step_b != i * step_a || bytes_a != bytes_b) return true;
+  }
+  return false;
 }
 
 // New rows of a sequence up to this many read the pages themselves, one by one; for more the pages are gathered first, once for

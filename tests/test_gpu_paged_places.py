@@ -38,13 +38,30 @@ def test_outputs_among_the_queries(hip, torch, stride, apart, dtype):  # noqa: F
     assert (buffer[~used] == 9.0).all()
 
 
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("q_at,q_stride,out_at,out_stride", [
-    (0, W, 0, W + 4), (0, 2 * W, 0, W), (0, W, 4, W), (0, W, W, W), (4, W, 0, W), (0, 2 * W, W - 4, 2 * W), (0, 2 * W, W + 4, 2 * W),
-    (0, W, 2 * W + 4, W), (W, W, 0, 2 * W)])
+    (0, 2 * W, W, 4 * W), (W, 4 * W, 0, 2 * W), (0, W, 5 * W, 2 * W), (0, 3 * W, W, W * 3 // 2 * 2), (10 * W, W, 0, 2 * W)])
+def test_outputs_between_queries_at_another_distance(hip, torch, q_at, q_stride, out_at, out_stride, dtype):  # noqa: F811
+    rng = np.random.default_rng(q_at + out_at)
+    ctx, lens = _ctx(hip, torch, H, KV, HD), [700, 3, 40, 70, 1300]
+    cache, held = _filled(hip, torch, ctx, lens, P, dtype, rng)
+    rows = rng.standard_normal((5, W)).astype(np.float32)
+    buffer = torch.full((24 * W,), 9.0, device="cuda")
+    q, out = _strided(torch, buffer, q_at, 5, q_stride), _strided(torch, buffer, out_at, 5, out_stride)
+    q.copy_(torch.from_numpy(rows))
+    ctx.attend_paged(cache, _ints(torch, range(5)), _ints(torch, [x - 1 for x in lens]), q, out=out)
+    ctx.sync()
+    _check_rows(out.cpu().numpy(), rows, held, range(5), [x - 1 for x in lens], HD)
+    assert np.array_equal(q.cpu().numpy(), rows)
+
+
+@pytest.mark.parametrize("q_at,q_stride,out_at,out_stride", [
+    (0, 2 * W, W, 3 * W), (0, 3 * W, 2 * W - 4, 4 * W), (4 * W, 2 * W, 0, W * 9 // 4), (0, W, 0, W + 4), (0, 2 * W, 0, W), (0, W, 4, W), (0, W, W, W), (4, W, 0, W), (0, 2 * W, W - 4, 2 * W), (0, 2 * W, W + 4, 2 * W),
+    (0, W, 2 * W + 4, W), (2 * W, W, 0, 2 * W)])
 def test_outputs_in_the_way_of_queries(hip, torch, q_at, q_stride, out_at, out_stride):  # noqa: F811
     ctx = _ctx(hip, torch, H, KV, HD)
     cache = hip.PagedKVCache(ctx, 4, P, 3, 2, dtype="f32")
-    buffer = torch.full((20 * W,), 9.0, device="cuda")
+    buffer = torch.full((24 * W,), 9.0, device="cuda")
     q, out = _strided(torch, buffer, q_at, 3, q_stride), _strided(torch, buffer, out_at, 3, out_stride)
     three = _ints(torch, [0, 1, 2])
     with pytest.raises(hip.ArgumentError, match="apart"):
